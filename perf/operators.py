@@ -136,7 +136,8 @@ def _codes(h13):
     halves = h13.reshape(2 * rows, width)
     blocks = _pad_blocks(halves).float()
     largest = blocks.abs().amax(-1, keepdim=True).clamp_min(1e-30)
-    codes = torch.round(blocks.double() * (127.0 / largest).double()).to(torch.int8)
+    factor = torch.full_like(largest, 127.0).div_(largest)  # (a number over a tensor is a reciprocal and a product)
+    codes = torch.round(blocks.double() * factor.double()).to(torch.int8)
     codes = codes.view(2 * rows, -1)[:, :width].reshape(rows, 2 * width)
     return codes, (largest / 127.0).view(rows, -1)
 
@@ -387,7 +388,7 @@ def exact(case, seed):
                 block = s["h13"][part, c:stop]
                 top = block.abs().amax(1, keepdim=True).float().clamp_min(1e-30)
                 # the kept form is defined by its two fp32 factors; the codes are whole numbers
-                codes = torch.round(block.double() * torch.div(127.0, top).double())
+                codes = torch.round(block.double() * (torch.full_like(top, 127.0) / top).double())
                 found["restored"][:, c:stop] = codes * torch.div(top, 127.0).double()
             names = ["act"] if case["form"] == "fp8" else []
         else:
