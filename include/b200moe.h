@@ -179,6 +179,33 @@ int b200moe_dswiglu_routed(const void* h13, long long ldh, const void* r, long l
                            float limit, int limited, int32_t* status, void* stream);
 
 /*
+ * The pre-activation kept in 8 bits between forward and backward: int8 codes [rows, 2*width] and one fp32
+ * scale per row, half (gate, up) and 128 columns of it, `2 * ceil(width / 128)` to a row, gate's first.  With
+ * a = max(largest magnitude of the block, 1e-30): code = rint(v * (127 / a)), scale = a / 127, value = code *
+ * scale.  A block with a NaN or an infinity has a NaN scale.  ld_codes in bytes, a multiple of 8.
+ *
+ * save8: b200moe_swiglu_quantize (same results, both of which may be NULL) that also writes codes and
+ * scales of h13 as it is, before any clamp.
+ * restore8: the bf16 values the codes stand for, [rows, 2*width].
+ * dswiglu_saved8: b200moe_dswiglu_routed on the values the codes stand for.
+ */
+int b200moe_swiglu_save8(const void* h13, long long ldh, long long rows, int width, void* act_q, long long ldq,
+                         float* scales, long long scale_row_stride, long long scale_block_stride, void* act_bf16,
+                         long long lda, void* codes, long long ld_codes, float* code_scales,
+                         long long code_scale_row_stride, long long code_scale_block_stride, float limit,
+                         int limited, void* stream);
+int b200moe_restore8(const void* codes, long long ld_codes, const float* code_scales,
+                     long long code_scale_row_stride, long long code_scale_block_stride, long long rows, int width,
+                     void* h13, long long ldh, void* stream);
+int b200moe_dswiglu_saved8(const void* codes, long long ld_codes, const float* code_scales,
+                           long long code_scale_row_stride, long long code_scale_block_stride, const void* r,
+                           long long ldr, const float* route_weights, long long n_weights, const int32_t* order,
+                           long long rows, int width, float* dscore, void* grad_h13_q, long long ldq,
+                           float* grad_h13_scales, long long scale_row_stride, long long scale_block_stride,
+                           void* grad_h13_bf16, long long ldg, void* act_scaled, long long lda, float limit,
+                           int limited, int32_t* status, void* stream);
+
+/*
  * Weight quantisation: w [experts, out, in] (bf16, or fp32 when src_is_fp32) ->
  * q E4M3 same shape, scale fp32 [experts, ceil(out/128), ceil(in/128)].
  * Reference: src/mlops/kernels/block_fp8.py:63-93 (`quantize_blocks`).
@@ -529,6 +556,15 @@ typedef struct b200moe_backward_args {
 } b200moe_backward_args;
 long long b200moe_backward_workspace_bytes(long long tokens, int width, int inner, int experts, int top_k);
 int b200moe_backward_fp8(const b200moe_backward_args* args, void* stream);
+
+/*
+ * The same two calls with h13 kept in 8 bits (b200moe_swiglu_save8): codes int8 [R, 2 inner] and code_scales
+ * fp32 [R, 2 inner / 128], dense.  In the forward call args->h13 is scratch, in the backward call it is not
+ * looked at.
+ */
+int b200moe_forward_fp8_save8(const b200moe_forward_args* args, void* codes, float* code_scales, void* stream);
+int b200moe_backward_fp8_saved8(const b200moe_backward_args* args, const void* codes, const float* code_scales,
+                                void* stream);
 
 /*
  * dst[slots[t * fanout + k], :] = src[t, :] (bf16 rows of `width`): b200moe_gather_rows with

@@ -69,6 +69,12 @@ SIGNATURES = {
         I,
         [P, LL, P, LL, P, LL, P, LL, I, P, P, LL, P, LL, LL, P, LL, P, LL, F, I, P, P],
     ),
+    "b200moe_swiglu_save8": (I, [P, LL, LL, I, P, LL, P, LL, LL, P, LL, P, LL, P, LL, LL, F, I, P]),
+    "b200moe_restore8": (I, [P, LL, P, LL, LL, LL, I, P, LL, P]),
+    "b200moe_dswiglu_saved8": (
+        I,
+        [P, LL, P, LL, LL, P, LL, P, LL, P, LL, I, P, P, LL, P, LL, LL, P, LL, P, LL, F, I, P, P],
+    ),
     "b200moe_quantize_blocks": (I, [P, I, I, I, I, P, P, P]),
     "b200moe_grouped_gemm_fp8": (
         I,
@@ -105,6 +111,8 @@ SIGNATURES = {
     "b200moe_forward_fp8": (I, [P, P]),
     "b200moe_backward_workspace_bytes": (LL, [LL, I, I, I, I]),
     "b200moe_backward_fp8": (I, [P, P]),
+    "b200moe_forward_fp8_save8": (I, [P, P, P, P]),
+    "b200moe_backward_fp8_saved8": (I, [P, P, P, P]),
     "b200moe_gather_scalar": (I, [P, LL, P, LL, P, P, P]),
 }
 

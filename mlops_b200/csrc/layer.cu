@@ -126,14 +126,17 @@ extern "C" long long b200moe_forward_workspace_bytes(long long tokens, int width
   return ForwardScratch(nullptr, tokens, width, inner, experts, top_k).bytes;
 }
 
-extern "C" int b200moe_forward_fp8(const b200moe_forward_args* a, void* stream) {
+// `codes`: h13 is kept in 8 bits and its bf16 buffer is scratch.
+static int forward_fp8(const b200moe_forward_args* a, bool save, void* codes, float* code_scales, void* stream) {
   if (a == nullptr || !sizes_ok(a->tokens, a->width, a->inner, a->experts, a->top_k) || !mode_ok(a->mode))
     return B200MOE_ERR_ARG;
   if (!all_given({a->x, a->residual, a->logits, a->w13, a->w13_scale, a->w2, a->w2_scale, a->route_weights, a->ids,
                   a->order, a->offsets, a->slots, a->counts, a->h13, a->output, a->aux, a->probability_sum, a->x_q,
-                  a->act_q, a->expert_rows, a->workspace, a->status}))
+                  a->act_q, a->expert_rows, a->workspace, a->status}) ||
+      (save && !all_given({codes, code_scales})))
     return B200MOE_ERR_ARG;
-  if (!all_aligned(16, {a->x, a->residual, a->w13, a->w2, a->h13, a->output, a->x_q, a->act_q, a->expert_rows}) ||
+  if (!all_aligned(16, {a->x, a->residual, a->w13, a->w2, a->h13, a->output, a->x_q, a->act_q, a->expert_rows,
+                        codes}) ||
       !all_aligned(256, {a->workspace}))
     return B200MOE_ERR_ALIGN;
   const int D = a->width, F = a->inner, E = a->experts, K = a->top_k;
@@ -148,8 +151,12 @@ extern "C" int b200moe_forward_fp8(const b200moe_forward_args* a, void* stream) 
             a->status, stream);
   B200_STEP(grouped_gemm_fp8, a->x_q, D, s.x_scale, 1, R, a->w13, a->w13_scale, a->h13, 2LL * F, nullptr, 0,
             a->offsets, E, E, R, 2 * F, D, 0, 256, a->status, stream);
-  B200_STEP(swiglu_quantize, a->h13, 2LL * F, R, F, a->act_q, F, s.act_scale, 1, R, nullptr, F, a->limit,
-            a->limited, stream);
+  if (save)
+    B200_STEP(swiglu_save8, a->h13, 2LL * F, R, F, a->act_q, F, s.act_scale, 1, R, nullptr, F, codes, 2LL * F,
+              code_scales, 2 * F / 128, 1, a->limit, a->limited, stream);
+  else
+    B200_STEP(swiglu_quantize, a->h13, 2LL * F, R, F, a->act_q, F, s.act_scale, 1, R, nullptr, F, a->limit,
+              a->limited, stream);
   B200_STEP(grouped_gemm_fp8, a->act_q, F, s.act_scale, 1, R, a->w2, a->w2_scale, a->expert_rows, D, nullptr, 0,
             a->offsets, E, E, R, D, F, 0, 256, a->status, stream);
   B200_STEP(combine, a->expert_rows, D, R, a->slots, a->route_weights, a->residual, D, a->output, D, T, D, K,
@@ -159,20 +166,29 @@ extern "C" int b200moe_forward_fp8(const b200moe_forward_args* a, void* stream) 
                                    reinterpret_cast<cudaStream_t>(stream));
 }
 
+extern "C" int b200moe_forward_fp8(const b200moe_forward_args* a, void* stream) {
+  return forward_fp8(a, false, nullptr, nullptr, stream);
+}
+
+extern "C" int b200moe_forward_fp8_save8(const b200moe_forward_args* a, void* codes, float* code_scales, void* stream) {
+  return forward_fp8(a, true, codes, code_scales, stream);
+}
+
 extern "C" long long b200moe_backward_workspace_bytes(long long tokens, int width, int inner, int experts, int top_k) {
   if (!sizes_ok(tokens, width, inner, experts, top_k)) return -1;
   return BackwardScratch(nullptr, tokens, width, inner, experts, top_k).bytes;
 }
 
-extern "C" int b200moe_backward_fp8(const b200moe_backward_args* a, void* stream) {
+static int backward_fp8(const b200moe_backward_args* a, bool saved, const void* codes, const float* code_scales,
+                        void* stream) {
   if (a == nullptr || !sizes_ok(a->tokens, a->width, a->inner, a->experts, a->top_k) || !mode_ok(a->mode))
     return B200MOE_ERR_ARG;
   if (!all_given({a->grad_output, a->x, a->w13, a->w13_scale, a->w2, a->w2_scale, a->logits, a->route_weights, a->ids,
-                  a->order, a->offsets, a->slots, a->h13, a->grad_x, a->grad_logits, a->grad_logits_high,
+                  a->order, a->offsets, a->slots, a->grad_x, a->grad_logits, a->grad_logits_high,
                   a->grad_logits_low, a->dy_q, a->rows, a->r, a->gh_q, a->workspace, a->status}) ||
-      (a->grad_w13 != nullptr && a->gh == nullptr))
+      (saved ? !all_given({codes, code_scales}) : a->h13 == nullptr) || (a->grad_w13 != nullptr && a->gh == nullptr))
     return B200MOE_ERR_ARG;
-  if (!all_aligned(16, {a->grad_output, a->x, a->w13, a->w2, a->h13, a->grad_x, a->grad_w13, a->grad_w2, a->dy_q,
+  if (!all_aligned(16, {a->grad_output, a->x, a->w13, a->w2, saved ? codes : a->h13, a->grad_x, a->grad_w13, a->grad_w2, a->dy_q,
                         a->rows, a->r, a->gh_q, a->gh}) ||
       !all_aligned(256, {a->workspace}))
     return B200MOE_ERR_ALIGN;
@@ -187,9 +203,14 @@ extern "C" int b200moe_backward_fp8(const b200moe_backward_args* a, void* stream
             dy_rows, D, a->status, stream);
   B200_STEP(grouped_gemm_fp8, a->dy_q, D, s.dy_scale, 1, R, a->w2, a->w2_scale, a->r, F, nullptr, 0, a->offsets,
             E, E, R, F, D, 1, 256, a->status, stream);
-  B200_STEP(dswiglu_routed, a->h13, 2LL * F, a->r, F, a->route_weights, R, a->order, R, F, s.dscore, a->gh_q,
-            2LL * F, s.gh_scale, 1, R, a->gh, 2LL * F, a->grad_w2 != nullptr ? a->r : nullptr, F,
-            a->limit, a->limited, a->status, stream);
+  void* act_scaled = a->grad_w2 != nullptr ? a->r : nullptr;
+  if (saved)
+    B200_STEP(dswiglu_saved8, codes, 2LL * F, code_scales, 2 * F / 128, 1, a->r, F, a->route_weights, R, a->order, R,
+              F, s.dscore, a->gh_q, 2LL * F, s.gh_scale, 1, R, a->gh, 2LL * F, act_scaled, F, a->limit, a->limited,
+              a->status, stream);
+  else
+    B200_STEP(dswiglu_routed, a->h13, 2LL * F, a->r, F, a->route_weights, R, a->order, R, F, s.dscore, a->gh_q,
+              2LL * F, s.gh_scale, 1, R, a->gh, 2LL * F, act_scaled, F, a->limit, a->limited, a->status, stream);
   B200_STEP(gather_scalar, s.dscore, R, a->slots, R, s.grad_route_weights, a->status, stream);
   if (a->grad_w2 != nullptr)
     B200_STEP(grouped_wgrad_bf16, a->rows, D, a->r, F, a->offsets, E, 1, R, D, F, a->grad_w2,
@@ -213,4 +234,13 @@ extern "C" int b200moe_backward_fp8(const b200moe_backward_args* a, void* stream
                                  a->grad_aux, a->grad_aux != nullptr ? s.frequency : nullptr,
                                  (float)((sigmoid ? 1.0 : (double)E) / (double)T), a->grad_probability_sum,
                                  a->grad_logits, E, a->grad_logits_high, a->grad_logits_low, cuda_stream);
+}
+
+extern "C" int b200moe_backward_fp8(const b200moe_backward_args* a, void* stream) {
+  return backward_fp8(a, false, nullptr, nullptr, stream);
+}
+
+extern "C" int b200moe_backward_fp8_saved8(const b200moe_backward_args* a, const void* codes,
+                                           const float* code_scales, void* stream) {
+  return backward_fp8(a, true, codes, code_scales, stream);
 }

@@ -34,6 +34,71 @@ __device__ __forceinline__ uint4 pack8_bf16(const float (&v)[8]) {
   return o;
 }
 
+// ---- the 8-bit form of a pre-activation row [gate | up] that a backward pass keeps ----
+// Per row, half and 128 columns: a = max(largest magnitude, 1e-30), code = rint(v * (127 / a)) as int8, scale =
+// a / 127; both quotients are rounded fp32 and the product is rounded once, to the whole number (ties to even).
+// What comes back, code * scale, is within a / 254 of the value.  int8 and not E4M3: a step of a / 127 is
+// 0.6% of the rms of a block of normal values, E4M3's three bits are 2.6% of it.  A block with a NaN or an infinity gets
+// a NaN scale and comes back as NaN.  Adding 1.5 * 2^23 leaves the whole number in a float's low bits, so a
+// code is one packed fma and a byte permute, and what is added back for the way out is exact.
+constexpr float kCodeFloor = 1e-30f;
+constexpr float kCodeMagic = 12582912.0f;  // 1.5 * 2^23
+
+__device__ __forceinline__ uint32_t max_u16x2(uint32_t a, uint32_t b) { return __vmaxu2(a, b); }
+
+// The magnitude bits of the largest of eight bf16 values (as integers they sort like the values, NaN on top).
+__device__ __forceinline__ uint32_t largest_bits(const uint4& raw) {
+  const uint32_t m = max_u16x2(max_u16x2(raw.x & 0x7fff7fffu, raw.y & 0x7fff7fffu),
+                               max_u16x2(raw.z & 0x7fff7fffu, raw.w & 0x7fff7fffu));
+  return max(m & 0xffffu, m >> 16);
+}
+
+struct CodeFactors {
+  float scale, inverse;
+};
+__device__ __forceinline__ CodeFactors code_factors(uint32_t bits) {
+  const float a = fmaxf(__uint_as_float(bits << 16), kCodeFloor);
+  if (bits >= 0x7f80u) return {__int_as_float(0x7fc00000), 0.0f};
+  return {__fdiv_rn(a, 127.0f), __fdiv_rn(127.0f, a)};
+}
+
+__device__ __forceinline__ uint2 encode8(const float (&v)[8], float inverse) {
+  const Float2 inv = splat2(inverse), magic = splat2(kCodeMagic);
+  uint32_t w[2];
+#pragma unroll
+  for (int i = 0; i < 8; i += 4) {
+    float a, b, c, d;
+    unpack2(mad2(pack2(v[i], v[i + 1]), inv, magic), a, b);
+    unpack2(mad2(pack2(v[i + 2], v[i + 3]), inv, magic), c, d);
+    w[i / 4] = __byte_perm(__byte_perm(__float_as_uint(a), __float_as_uint(b), 0x0040),
+                           __byte_perm(__float_as_uint(c), __float_as_uint(d), 0x0040), 0x5410);
+  }
+  return make_uint2(w[0], w[1]);
+}
+
+__device__ __forceinline__ void decode8(const uint2& codes, float scale, float (&v)[8]) {
+  const Float2 one = splat2(1.0f), back = splat2(-8388736.0f), factor = splat2(scale);  // 2^23 + 128
+#pragma unroll
+  for (int i = 0; i < 8; i += 4) {
+    const uint32_t w = (i == 0 ? codes.x : codes.y) ^ 0x80808080u;  // code + 128
+#pragma unroll
+    for (int j = 0; j < 4; j += 2) {
+      const float a = __uint_as_float(__byte_perm(w, 0x4b000000u, 0x7440 + j));
+      const float b = __uint_as_float(__byte_perm(w, 0x4b000000u, 0x7440 + j + 1));
+      unpack2(mul2(mad2(pack2(a, b), one, back), factor), v[i + j], v[i + j + 1]);
+    }
+  }
+}
+
+// Where the codes of [gate | up] rows are: row pitch `ld`, scale of (row, half, block) at
+// r * s_row + (half * blocks of a half + block) * s_block.
+struct SavedRows {
+  int8_t* codes;
+  long long ld;
+  float* scales;
+  long long s_row, s_block;
+};
+
 // mode 0: one scale per 128-column block.  mode 1: one scale per row (two passes).
 __global__ void __launch_bounds__(kRowWarps * 32)
 quantize_rows_kernel(const __nv_bfloat16* __restrict__ x, long long ldx, long long src_rows,
@@ -162,17 +227,18 @@ quantize_scatter_kernel(const __nv_bfloat16* __restrict__ x, long long ldx, long
 
 // act = silu(gate) * up computed in fp32 from h13 = [gate | up] (each F wide), rounded
 // once: to E4M3 with 1x128 scales (act_q / scales) and, when act_bf16 is given, to bf16.
+// SAVED: the pre-activation is kept in 8 bits as well (before any clamp), from the registers that hold it.
 // Optional GLM clamp: gate capped at `limit`, up clipped to [-limit, limit].
 // One warp per `per_warp` consecutive pieces of 256 columns of a row: the next piece is loaded
 // while one is worked on.  Issue-bound in its arithmetic: with the library's rounded reciprocal and scalar
 // arithmetic 32768 rows of F = 14336 took 0.61 ms, with sigmoid8 and packed arithmetic 0.475 (5.0 TB/s);
 // 512 rows of F = 2048 take 4.1 us instead of 10.
-template <bool LIMITED>
+template <bool LIMITED, bool SAVED>
 __global__ void __launch_bounds__(kRowWarps * 32)
 swiglu_quant_kernel(const __nv_bfloat16* __restrict__ h13, long long ldh, long long rows, int F,
                     uint8_t* __restrict__ act_q, long long ldq, float* __restrict__ scales,
                     long long s_row, long long s_kb, __nv_bfloat16* __restrict__ act_bf16,
-                    long long lda, float limit, int per_warp, int warps_per_row) {
+                    long long lda, float limit, int per_warp, int warps_per_row, SavedRows saved) {
   const int lane = threadIdx.x & 31;
   const long long w = (long long)blockIdx.x * kRowWarps + (threadIdx.x >> 5);
   const long long r = w / warps_per_row;
@@ -193,6 +259,22 @@ swiglu_quant_kernel(const __nv_bfloat16* __restrict__ h13, long long ldh, long l
     float g[8], u[8], a[8], sig[8];
     unpack8(rg, g);
     unpack8(ru, u);
+    if constexpr (SAVED) {  // both halves' largest magnitudes in one exchange
+      uint32_t m = largest_bits(rg) | (largest_bits(ru) << 16);
+#pragma unroll
+      for (int o = 8; o > 0; o >>= 1) m = max_u16x2(m, __shfl_xor_sync(0xffffffffu, m, o));
+      const CodeFactors fg = code_factors(m & 0xffffu), fu = code_factors(m >> 16);
+      if (c < F) {
+        int8_t* code = saved.codes + r * saved.ld + c;
+        *reinterpret_cast<uint2*>(code) = encode8(g, fg.inverse);
+        *reinterpret_cast<uint2*>(code + F) = encode8(u, fu.inverse);
+        if ((lane & 15) == 0) {
+          float* scale = saved.scales + r * saved.s_row + (long long)(c >> 7) * saved.s_block;
+          scale[0] = fg.scale;
+          scale[(long long)((F + 127) >> 7) * saved.s_block] = fu.scale;
+        }
+      }
+    }
     fetch(c + 256);
     if constexpr (LIMITED) {
 #pragma unroll
@@ -237,7 +319,7 @@ swiglu_quant_kernel(const __nv_bfloat16* __restrict__ h13, long long ldh, long l
 // scalar arithmetic, which kept the kernel issue-bound.  Three blocks to an SM need 80 registers a
 // thread; at the 83 the compiler takes unasked two fit, and the same took 1.20 ms.  (With a limit 80
 // would spill.)
-template <bool LIMITED>
+template <bool LIMITED, bool SAVED>
 __global__ void __launch_bounds__(kRowWarps * 32, LIMITED ? 2 : 3)
 dswiglu_routed_kernel(const __nv_bfloat16* h13, long long ldh,  // may be the same buffer as gh_bf16
                       const __nv_bfloat16* rmat, long long ldr,       // may be the same buffer as act_scaled
@@ -246,18 +328,36 @@ dswiglu_routed_kernel(const __nv_bfloat16* h13, long long ldh,  // may be the sa
                       uint8_t* __restrict__ gh_q, long long ldq, float* __restrict__ gh_scales,
                       long long s_row, long long s_kb, __nv_bfloat16* gh_bf16,
                       long long ldg, __nv_bfloat16* act_scaled, long long lda, float limit,
-                      int* status) {
+                      SavedRows saved, int* status) {
   const int lane = threadIdx.x & 31;
   const long long r = (long long)blockIdx.x * kRowWarps + (threadIdx.x >> 5);
   if (r >= rows) return;
   const __nv_bfloat16* hr = h13 + r * ldh;
   const __nv_bfloat16* rr = rmat + r * ldr;
-  uint4 rg, ru, rx;
+  uint4 rx;
+  uint4 rg, ru;    // sixteen bf16 values of h13, or
+  uint2 qg, qu;    // their codes
+  float sg8, su8;  // and scales
   auto fetch = [&](int c) {
-    rg = ru = rx = make_uint4(0, 0, 0, 0);
+    rx = make_uint4(0, 0, 0, 0);
+    if constexpr (SAVED) {
+      qg = qu = make_uint2(0, 0);
+      sg8 = su8 = 0.f;
+    } else {
+      rg = ru = make_uint4(0, 0, 0, 0);
+    }
     if (c < F) {
-      rg = *reinterpret_cast<const uint4*>(hr + c);
-      ru = *reinterpret_cast<const uint4*>(hr + F + c);
+      if constexpr (SAVED) {
+        const int8_t* code = saved.codes + r * saved.ld + c;
+        qg = *reinterpret_cast<const uint2*>(code);
+        qu = *reinterpret_cast<const uint2*>(code + F);
+        const float* scale = saved.scales + r * saved.s_row + (long long)(c >> 7) * saved.s_block;
+        sg8 = scale[0];
+        su8 = scale[(long long)((F + 127) >> 7) * saved.s_block];
+      } else {
+        rg = *reinterpret_cast<const uint4*>(hr + c);
+        ru = *reinterpret_cast<const uint4*>(hr + F + c);
+      }
       rx = *reinterpret_cast<const uint4*>(rr + c);
     }
   };
@@ -274,8 +374,13 @@ dswiglu_routed_kernel(const __nv_bfloat16* h13, long long ldh,  // may be the sa
     const int c = c0 + lane * 8;
     float g[8], u[8], rv[8], dg[8], du[8], sig[8];
     uint32_t scaled[4];  // score * act
-    unpack8(rg, g);
-    unpack8(ru, u);
+    if constexpr (SAVED) {
+      decode8(qg, sg8, g);
+      decode8(qu, su8, u);
+    } else {
+      unpack8(rg, g);
+      unpack8(ru, u);
+    }
     unpack8(rx, rv);
     fetch(c + 256);
     uint32_t keep_g = 0xff, keep_u = 0xff;
@@ -337,6 +442,23 @@ dswiglu_routed_kernel(const __nv_bfloat16* h13, long long ldh,  // may be the sa
   }
   dot = warp_sum(dot);
   if (lane == 0 && dscore != nullptr) dscore[r] = dot;
+}
+
+// bf16 values of kept rows, eight columns of a half per thread.  Bound by HBM (2 bytes in, 4 out per column pair).
+__global__ void __launch_bounds__(256)
+restore_kernel(SavedRows saved, long long rows, int F, __nv_bfloat16* __restrict__ out, long long ldo) {
+  const int chunks = F / 8;  // of a half
+  const long long total = rows * 2 * chunks;
+  for (long long i = (long long)blockIdx.x * blockDim.x + threadIdx.x; i < total; i += (long long)gridDim.x * blockDim.x) {
+    const long long rh = i / chunks;
+    const int c = (int)(i - rh * chunks) * 8, half = (int)(rh & 1);
+    const long long r = rh >> 1;
+    const uint2 code = *reinterpret_cast<const uint2*>(saved.codes + r * saved.ld + half * F + c);
+    const float scale = saved.scales[r * saved.s_row + (long long)(half * ((F + 127) >> 7) + (c >> 7)) * saved.s_block];
+    float v[8];
+    decode8(code, scale, v);
+    *reinterpret_cast<uint4*>(out + r * ldo + half * F + c) = pack8_bf16(v);
+  }
 }
 
 // One CTA per 128x128 block of a [E, out, in] weight (bf16 or fp32 source), read ONCE: 512 threads
@@ -634,12 +756,10 @@ extern "C" int b200moe_quantize_rows_scatter(const void* x, long long ldx, long 
   return launch_status();
 }
 
-extern "C" int b200moe_swiglu_quantize(const void* h13, long long ldh, long long rows, int width,
-                                       void* act_q, long long ldq, float* scales,
-                                       long long scale_row_stride, long long scale_block_stride,
-                                       void* act_bf16, long long lda, float limit, int limited,
-                                       void* stream) {
-  if (!h13 || rows < 0 || width <= 0 || (!act_q && !act_bf16) || (act_q && !scales)) return B200MOE_ERR_ARG;
+static int launch_swiglu(const void* h13, long long ldh, long long rows, int width, void* act_q, long long ldq,
+                         float* scales, long long scale_row_stride, long long scale_block_stride, void* act_bf16,
+                         long long lda, const SavedRows* saved, float limit, int limited, void* stream) {
+  if (!h13 || rows < 0 || width <= 0 || (act_q && !scales)) return B200MOE_ERR_ARG;
   if ((width % 8) || (ldh % 8) || (ldq % 8) || (lda % 8) || ((uintptr_t)h13 & 15) || ((uintptr_t)act_q & 7) ||
       ((uintptr_t)act_bf16 & 15))
     return B200MOE_ERR_ALIGN;
@@ -648,11 +768,81 @@ extern "C" int b200moe_swiglu_quantize(const void* h13, long long ldh, long long
   const int chunks = (width + 255) / 256;
   const int per_warp = rows >= 32LL * sm_count_device() ? chunks : 1;
   const int warps_per_row = (chunks + per_warp - 1) / per_warp;
-  auto kern = limited ? swiglu_quant_kernel<true> : swiglu_quant_kernel<false>;
+  auto kern = saved != nullptr ? (limited ? swiglu_quant_kernel<true, true> : swiglu_quant_kernel<false, true>)
+                               : (limited ? swiglu_quant_kernel<true, false> : swiglu_quant_kernel<false, false>);
   kern<<<row_grid(rows * warps_per_row), kRowWarps * 32, 0, reinterpret_cast<cudaStream_t>(stream)>>>(
       reinterpret_cast<const __nv_bfloat16*>(h13), ldh, rows, width, reinterpret_cast<uint8_t*>(act_q), ldq, scales,
       scale_row_stride, scale_block_stride, reinterpret_cast<__nv_bfloat16*>(act_bf16), lda, limit, per_warp,
-      warps_per_row);
+      warps_per_row, saved != nullptr ? *saved : SavedRows{});
+  return launch_status();
+}
+
+extern "C" int b200moe_swiglu_quantize(const void* h13, long long ldh, long long rows, int width,
+                                       void* act_q, long long ldq, float* scales,
+                                       long long scale_row_stride, long long scale_block_stride,
+                                       void* act_bf16, long long lda, float limit, int limited,
+                                       void* stream) {
+  if (!act_q && !act_bf16) return B200MOE_ERR_ARG;
+  return launch_swiglu(h13, ldh, rows, width, act_q, ldq, scales, scale_row_stride, scale_block_stride, act_bf16, lda,
+                       nullptr, limit, limited, stream);
+}
+
+static int check_saved(const SavedRows& s, long long rows, int width) {
+  if (!s.codes || !s.scales || rows < 0 || width <= 0) return B200MOE_ERR_ARG;
+  if ((width % 8) || (s.ld % 8) || ((uintptr_t)s.codes & 7) || ((uintptr_t)s.scales & 3)) return B200MOE_ERR_ALIGN;
+  return B200MOE_OK;
+}
+
+extern "C" int b200moe_swiglu_save8(const void* h13, long long ldh, long long rows, int width, void* act_q,
+                                    long long ldq, float* scales, long long scale_row_stride,
+                                    long long scale_block_stride, void* act_bf16, long long lda, void* codes,
+                                    long long ld_codes, float* code_scales, long long code_scale_row_stride,
+                                    long long code_scale_block_stride, float limit, int limited, void* stream) {
+  const SavedRows saved = {reinterpret_cast<int8_t*>(codes), ld_codes, code_scales, code_scale_row_stride,
+                           code_scale_block_stride};
+  const int code = check_saved(saved, rows, width);
+  if (code != B200MOE_OK) return code;
+  return launch_swiglu(h13, ldh, rows, width, act_q, ldq, scales, scale_row_stride, scale_block_stride, act_bf16, lda,
+                       &saved, limit, limited, stream);
+}
+
+extern "C" int b200moe_restore8(const void* codes, long long ld_codes, const float* code_scales,
+                                long long code_scale_row_stride, long long code_scale_block_stride, long long rows,
+                                int width, void* h13, long long ldh, void* stream) {
+  const SavedRows saved = {(int8_t*)codes, ld_codes, (float*)code_scales, code_scale_row_stride,
+                           code_scale_block_stride};
+  const int code = check_saved(saved, rows, width);
+  if (code != B200MOE_OK) return code;
+  if (!h13) return B200MOE_ERR_ARG;
+  if ((ldh % 8) || ((uintptr_t)h13 & 15)) return B200MOE_ERR_ALIGN;
+  if (rows == 0) return B200MOE_OK;
+  const long long blocks = (rows * (width / 4) + 255) / 256, most = 16LL * sm_count_device();
+  restore_kernel<<<(unsigned)(blocks < most ? blocks : most), 256, 0, reinterpret_cast<cudaStream_t>(stream)>>>(
+      saved, rows, width, reinterpret_cast<__nv_bfloat16*>(h13), ldh);
+  return launch_status();
+}
+
+static int launch_dswiglu(const void* h13, long long ldh, const SavedRows* saved, const void* r, long long ldr,
+                          const float* route_weights, long long n_weights, const int32_t* order, long long rows,
+                          int width, float* dscore, void* grad_h13_q, long long ldq, float* grad_h13_scales,
+                          long long scale_row_stride, long long scale_block_stride, void* grad_h13_bf16,
+                          long long ldg, void* act_scaled, long long lda, float limit, int limited, int32_t* status,
+                          void* stream) {
+  if (!r || !route_weights || !order || !status || rows < 0 || width <= 0) return B200MOE_ERR_ARG;
+  if (rows > 0 && n_weights <= 0) return B200MOE_ERR_ARG;
+  if (grad_h13_q && !grad_h13_scales) return B200MOE_ERR_ARG;
+  if ((width % 8) || (ldh % 8) || (ldr % 8) || (ldq % 8) || (ldg % 8) || (lda % 8)) return B200MOE_ERR_ALIGN;
+  if (((uintptr_t)h13 & 15) || ((uintptr_t)r & 15) || ((uintptr_t)grad_h13_q & 7) ||
+      ((uintptr_t)grad_h13_bf16 & 15) || ((uintptr_t)act_scaled & 15))
+    return B200MOE_ERR_ALIGN;
+  if (rows == 0) return B200MOE_OK;
+  auto kern = saved != nullptr ? (limited ? dswiglu_routed_kernel<true, true> : dswiglu_routed_kernel<false, true>)
+                               : (limited ? dswiglu_routed_kernel<true, false> : dswiglu_routed_kernel<false, false>);
+  kern<<<row_grid(rows), kRowWarps * 32, 0, reinterpret_cast<cudaStream_t>(stream)>>>(
+      reinterpret_cast<const __nv_bfloat16*>(h13), ldh, reinterpret_cast<const __nv_bfloat16*>(r), ldr,
+      route_weights, n_weights, order, rows, width, dscore, reinterpret_cast<uint8_t*>(grad_h13_q), ldq,
+      grad_h13_scales, scale_row_stride, scale_block_stride, reinterpret_cast<__nv_bfloat16*>(grad_h13_bf16), ldg,
+      reinterpret_cast<__nv_bfloat16*>(act_scaled), lda, limit, saved != nullptr ? *saved : SavedRows{}, status);
   return launch_status();
 }
 
@@ -663,21 +853,27 @@ extern "C" int b200moe_dswiglu_routed(const void* h13, long long ldh, const void
                                       long long scale_block_stride, void* grad_h13_bf16, long long ldg,
                                       void* act_scaled, long long lda, float limit, int limited,
                                       int32_t* status, void* stream) {
-  if (!h13 || !r || !route_weights || !order || !status || rows < 0 || width <= 0) return B200MOE_ERR_ARG;
-  if (rows > 0 && n_weights <= 0) return B200MOE_ERR_ARG;
-  if (grad_h13_q && !grad_h13_scales) return B200MOE_ERR_ARG;
-  if ((width % 8) || (ldh % 8) || (ldr % 8) || (ldq % 8) || (ldg % 8) || (lda % 8)) return B200MOE_ERR_ALIGN;
-  if (((uintptr_t)h13 & 15) || ((uintptr_t)r & 15) || ((uintptr_t)grad_h13_q & 7) ||
-      ((uintptr_t)grad_h13_bf16 & 15) || ((uintptr_t)act_scaled & 15))
-    return B200MOE_ERR_ALIGN;
-  if (rows == 0) return B200MOE_OK;
-  auto kern = limited ? dswiglu_routed_kernel<true> : dswiglu_routed_kernel<false>;
-  kern<<<row_grid(rows), kRowWarps * 32, 0, reinterpret_cast<cudaStream_t>(stream)>>>(
-      reinterpret_cast<const __nv_bfloat16*>(h13), ldh, reinterpret_cast<const __nv_bfloat16*>(r), ldr,
-      route_weights, n_weights, order, rows, width, dscore, reinterpret_cast<uint8_t*>(grad_h13_q), ldq,
-      grad_h13_scales, scale_row_stride, scale_block_stride, reinterpret_cast<__nv_bfloat16*>(grad_h13_bf16), ldg,
-      reinterpret_cast<__nv_bfloat16*>(act_scaled), lda, limit, status);
-  return launch_status();
+  if (!h13) return B200MOE_ERR_ARG;
+  return launch_dswiglu(h13, ldh, nullptr, r, ldr, route_weights, n_weights, order, rows, width, dscore, grad_h13_q,
+                        ldq, grad_h13_scales, scale_row_stride, scale_block_stride, grad_h13_bf16, ldg, act_scaled,
+                        lda, limit, limited, status, stream);
+}
+
+extern "C" int b200moe_dswiglu_saved8(const void* codes, long long ld_codes, const float* code_scales,
+                                      long long code_scale_row_stride, long long code_scale_block_stride,
+                                      const void* r, long long ldr, const float* route_weights, long long n_weights,
+                                      const int32_t* order, long long rows, int width, float* dscore,
+                                      void* grad_h13_q, long long ldq, float* grad_h13_scales,
+                                      long long scale_row_stride, long long scale_block_stride, void* grad_h13_bf16,
+                                      long long ldg, void* act_scaled, long long lda, float limit, int limited,
+                                      int32_t* status, void* stream) {
+  const SavedRows saved = {(int8_t*)codes, ld_codes, (float*)code_scales, code_scale_row_stride,
+                           code_scale_block_stride};
+  const int code = check_saved(saved, rows, width);
+  if (code != B200MOE_OK) return code;
+  return launch_dswiglu(nullptr, 0, &saved, r, ldr, route_weights, n_weights, order, rows, width, dscore, grad_h13_q,
+                        ldq, grad_h13_scales, scale_row_stride, scale_block_stride, grad_h13_bf16, ldg, act_scaled,
+                        lda, limit, limited, status, stream);
 }
 
 // E4M3 rows of x [rows, width] with one scale per (group, column): scales [groups, width].

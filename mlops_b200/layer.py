@@ -23,6 +23,7 @@ import torch
 from . import ops
 
 BLOCK_N_DEFAULT = 256
+SAVED_FORMS = ("bf16", "int8")  # of the pre-activation between forward and backward
 
 
 # ------------------------------------------------------------------------- router GEMM
@@ -136,6 +137,7 @@ def forward_routed(
     route: tuple[torch.Tensor, torch.Tensor] | None = None,
     fuse_swiglu: bool = False,
     fuse_combine: bool = False,
+    saved: str = "bf16",
 ) -> tuple[torch.Tensor, ...]:
     """Returns `(output, aux, counts, probability_sum, logits, route_weights, route_ids,
     order, offsets, slots, h13)`.
@@ -151,7 +153,14 @@ def forward_routed(
     by default). `fuse_combine` forms the route-weighted sum in the down GEMM's store with fp32
     atomics instead of writing expert-order rows for `combine`: not bitwise repeatable, and
     slower for top-8 routing (a token row is read-modify-written eight times in HBM), so it is
-    off by default as well."""
+    off by default as well. `saved="int8"` keeps the pre-activation for the backward pass in half the
+    bytes: the last entry is then `(codes, code_scales)` (`ops.swiglu_save8`), which `backward_routed` takes
+    in the place of h13; every other result is the same, bit for bit."""
+    if saved not in SAVED_FORMS:
+        raise ValueError("saved is 'bf16' or 'int8'")
+    save8 = saved == "int8"
+    if save8 and fuse_swiglu:
+        raise ValueError("fuse_swiglu keeps h13 in bf16: the 8-bit form is written by the separate SwiGLU pass")
     bf16_weights = isinstance(w13, torch.Tensor)
     if bf16_weights:
         _check_bf16_weights(w13, w2)
@@ -176,7 +185,7 @@ def forward_routed(
             output, aux, counts, probability_sum, *residuals = ops.forward_fp8(
                 h2_flat, residual_flat, logits, w13, w2, top_k=int(top_k), mode=str(routing_mode), bias=bias,
                 n_group=int(n_group), topk_group=int(topk_group), routed_scaling=float(routed_scaling),
-                limit=None if swiglu_limit is None else float(swiglu_limit))
+                limit=None if swiglu_limit is None else float(swiglu_limit), save8=save8)
             return (output.reshape(original_shape), aux, counts, probability_sum, logits, *residuals)
         if route is None:
             bias = None if router_bias is None or router_bias.numel() == 0 else router_bias
@@ -199,7 +208,7 @@ def forward_routed(
             x_rows = expert_rows(h2_flat, order, slots, int(top_k))
             h13 = ops.grouped_gemm_bf16(x_rows, w13_data, offsets)
             del x_rows
-            _q, _s, act = ops.swiglu_quantize(h13, limit=swiglu_limit, quantized=False, rounded=True)
+            _q, _s, act, h13 = _swiglu(h13, save8, limit=swiglu_limit, quantized=False, rounded=True)
             expert_output = ops.grouped_gemm_bf16(act, w2_data, offsets)
             output = ops.combine(expert_output, slots, route_weights, residual_flat).reshape(original_shape)
             aux, counts, probability_sum = routing_statistics(
@@ -213,7 +222,7 @@ def forward_routed(
             h13, a_q, a_s = ops.grouped_gemm_fp8_swiglu(x_q, x_s, w13_data, w13_scale, offsets, limit=swiglu_limit)
         else:
             h13 = ops.grouped_gemm_fp8(x_q, x_s, w13_data, w13_scale, offsets, block_n=block_n)
-            a_q, a_s, _ = ops.swiglu_quantize(h13, limit=swiglu_limit)
+            a_q, a_s, _, h13 = _swiglu(h13, save8, limit=swiglu_limit)
         if fuse_combine:
             output = ops.grouped_gemm_fp8_combine(
                 a_q, a_s, w2_data, w2_scale, offsets, order, route_weights, h2_flat.shape[0],
@@ -225,6 +234,20 @@ def forward_routed(
             logits, route_ids, counts, routing_mode=str(routing_mode), lengths=normalized, experts=experts
         )
     return (output, aux, counts, probability_sum, logits, route_weights, route_ids, order, offsets, slots, h13)
+
+
+def _swiglu(h13, save8, **kwargs):
+    """SwiGLU and what is kept of its input: `(act_q, scales, act_bf16, kept)`."""
+    if save8:
+        return ops.swiglu_save8(h13, **kwargs)
+    return *ops.swiglu_quantize(h13, **kwargs), h13
+
+
+def _dswiglu(kept, *args, **kwargs):
+    """The routed SwiGLU backward on h13 or on its 8-bit form."""
+    if isinstance(kept, torch.Tensor):
+        return ops.dswiglu_routed(kept, *args, **kwargs)
+    return ops.dswiglu_saved8(kept, *args, **kwargs)
 
 
 def expert_rows(x, order, slots, top_k):
@@ -276,7 +299,7 @@ def backward_routed(
     order: torch.Tensor,
     offsets: torch.Tensor,
     slots: torch.Tensor,
-    h13: torch.Tensor,
+    h13: torch.Tensor | tuple[torch.Tensor, torch.Tensor],
     *,
     top_k: int,
     routing_mode: str,
@@ -297,7 +320,8 @@ def backward_routed(
     bf16-operand products with fp32 sums, written at `weight_grad_dtype` (bf16 when None).
     `weight_grad_operands="fp8"` selects the reference's optional FP8 weight-gradient recipe
     instead (src/mlops/kernels/quack_moe/wgrad.py:30-69): both operands of each product are
-    quantised to E4M3 with one scale per expert and column and multiplied at the FP8 rate."""
+    quantised to E4M3 with one scale per expert and column and multiplied at the FP8 rate.
+    `h13` is the forward pass's last result, the bf16 tensor or its 8-bit form."""
     if weight_grad_operands not in ("bf16", "fp8"):
         raise ValueError("weight_grad_operands is 'bf16' or 'fp8'")
     bf16_weights = isinstance(w13, torch.Tensor)
@@ -336,7 +360,7 @@ def backward_routed(
         if bf16_weights:
             dy_rows = expert_rows(grad_flat, order, slots, int(top_k))
             r = ops.grouped_gemm_bf16(dy_rows, w2_data, offsets, b_mn_major=True)
-            dscore, _gq, _gs, gh_b, act_scaled = ops.dswiglu_routed(
+            dscore, _gq, _gs, gh_b, act_scaled = _dswiglu(
                 h13, r, route_weights, order, limit=swiglu_limit, quantized=False, rounded=True,
                 scaled_activation=need_w2,
             )
@@ -368,7 +392,7 @@ def backward_routed(
         else:
             dy_q, dy_s = ops.quantize_rows_scatter(grad_flat, slots)
         r = ops.grouped_gemm_fp8(dy_q, dy_s, w2_data, w2_scale, offsets, b_mn_major=True, block_n=block_n)
-        dscore, gh_q, gh_s, gh_b, act_scaled = ops.dswiglu_routed(
+        dscore, gh_q, gh_s, gh_b, act_scaled = _dswiglu(
             h13, r, route_weights, order, limit=swiglu_limit, quantized=True, rounded=need_w13,
             scaled_activation=need_w2,
         )
@@ -401,7 +425,9 @@ def _saved_as_formed(x, dy, logits, route_weights, route_ids, order, offsets, sl
             and ops.dense(route_weights, torch.float32, tokens, top_k)
             and ops.dense(route_ids, torch.int32, tokens, top_k) and ops.dense(order, torch.int32, rows)
             and ops.dense(offsets, torch.int32, experts + 1) and ops.dense(slots, torch.int32, tokens, top_k)
-            and ops.dense(h13, torch.bfloat16, rows, 2 * inner))
+            and (ops.dense(h13, torch.bfloat16, rows, 2 * inner) if isinstance(h13, torch.Tensor)
+                 else ops.dense(h13[0], torch.int8, rows, 2 * inner)
+                 and ops.dense(h13[1], torch.float32, rows, 2 * inner // 128)))
 
 
 def _finish_backward(grad_h2, grad_output, grad_aux, grad_probability_sum, grad_route_weights, route_weights,

@@ -415,6 +415,124 @@ def dswiglu_routed(h13, r, route_weights, order, *, limit=None, quantized=True, 
     return dscore, gq, gs, gb, a_s
 
 
+# -------------------------------------------------- the pre-activation kept in 8 bits for the backward pass
+def _saved_blocks(width):
+    return 2 * ((width + 127) // 128)
+
+
+def _check_saved(codes, scales):
+    """`(rows, width)` of kept rows; their layout is what `swiglu_save8` writes, with any row pitch."""
+    if (codes.dtype != torch.int8 or codes.dim() != 2 or codes.shape[1] % 16 or codes.shape[1] == 0
+            or (codes.shape[0] > 0 and codes.stride(1) != 1)):
+        raise NativeError("kept rows are int8 [rows, 2F] with unit inner stride, F a multiple of 8")
+    rows, width = codes.shape[0], codes.shape[1] // 2
+    if scales.dtype != torch.float32 or tuple(scales.shape) != (rows, _saved_blocks(width)):
+        raise NativeError(f"their scales are fp32 [rows, 2 ceil(F / 128)] = [{rows}, {_saved_blocks(width)}]")
+    return rows, width
+
+
+@_on_tensor_device
+def swiglu_save8(h13, *, limit=None, quantized=True, rounded=False):
+    """`swiglu_quantize` that also keeps h13 for the backward pass in 8 bits: `(act_q, scales, act_bf16,
+    (codes, code_scales))`, codes int8 `[rows, 2F]` and one fp32 scale per row, half and 128 columns
+    (`[rows, 2 ceil(F / 128)]`, gate's first). The kept values, `restore8((codes, code_scales))`, are within
+    1/254 of a block's largest magnitude; a block with a NaN or an infinity comes back as NaN. The activation
+    is that of `swiglu_quantize`, bit for bit."""
+    device = _need_cuda(h13)
+    if h13.dtype != torch.bfloat16 or h13.dim() != 2 or h13.shape[1] % 16 or h13.shape[1] == 0 \
+            or (h13.shape[0] > 0 and h13.stride(1) != 1):
+        raise NativeError("h13 must be bf16 [rows, 2F] with unit inner stride, F a multiple of 8")
+    rows, two_f = h13.shape
+    width = two_f // 2
+    act_q = scales = act = None
+    if quantized:
+        act_q = torch.empty((rows, width), dtype=FP8, device=device)
+        scales = _scale_buffer(rows, (width + 127) // 128, device)
+    if rounded:
+        act = torch.empty((rows, width), dtype=torch.bfloat16, device=device)
+    codes = torch.empty((rows, two_f), dtype=torch.int8, device=device)
+    code_scales = torch.empty((rows, _saved_blocks(width)), dtype=torch.float32, device=device)
+    if rows:
+        check(
+            lib.b200moe_swiglu_save8(
+                h13.data_ptr(), h13.stride(0), rows, width, _ptr(act_q), width, _ptr(scales),
+                0 if scales is None else scales.stride(0), 0 if scales is None else scales.stride(1),
+                _ptr(act), width, codes.data_ptr(), codes.stride(0), code_scales.data_ptr(), code_scales.stride(0),
+                code_scales.stride(1), 0.0 if limit is None else float(limit), 0 if limit is None else 1, _stream(),
+            ),
+            "swiglu_save8",
+        )
+        _count()
+    return act_q, scales, act, (codes, code_scales)
+
+
+def restore8(saved):
+    """bf16 `[rows, 2F]`: the pre-activation `swiglu_save8` kept."""
+    return _restore8(*saved)
+
+
+@_on_tensor_device
+def _restore8(codes, code_scales):
+    device = _need_cuda(codes, code_scales)
+    rows, width = _check_saved(codes, code_scales)
+    out = torch.empty((rows, 2 * width), dtype=torch.bfloat16, device=device)
+    if rows:
+        check(
+            lib.b200moe_restore8(codes.data_ptr(), codes.stride(0), code_scales.data_ptr(), code_scales.stride(0),
+                                 code_scales.stride(1), rows, width, out.data_ptr(), out.stride(0), _stream()),
+            "restore8",
+        )
+        _count()
+    return out
+
+
+def dswiglu_saved8(saved, r, route_weights, order, *, limit=None, quantized=True, rounded=False,
+                   scaled_activation=False):
+    """`dswiglu_routed` on the pre-activation `swiglu_save8` kept, read in its 8 bits: `(dscore [rows] fp32,
+    grad_h13_q, grad_h13_scales, grad_h13_bf16, act_scaled)`. The gradient is that of SwiGLU at the kept
+    values; with a limit, what is clamped goes by them too."""
+    return _dswiglu_saved8(*saved, r, route_weights, order, limit, quantized, rounded, scaled_activation)
+
+
+@_on_tensor_device
+def _dswiglu_saved8(codes, code_scales, r, route_weights, order, limit, quantized, rounded, scaled_activation):
+    device = _need_cuda(codes, code_scales, r, route_weights, order)
+    rows, width = _check_saved(codes, code_scales)
+    if r.dtype != torch.bfloat16 or tuple(r.shape) != (rows, width) or (rows > 0 and r.stride(1) != 1):
+        raise NativeError(f"r must be bf16 [{rows}, {width}] with unit inner stride")
+    if quantized and width % 128:
+        raise NativeError("the E4M3 gradient needs F to be a multiple of 128")
+    if order.dtype != torch.int32 or not order.is_contiguous() or order.numel() != rows:
+        raise NativeError("order must be contiguous int32 with one entry per row")
+    weights = route_weights.reshape(-1)
+    if weights.dtype != torch.float32 or (rows > 0 and weights.numel() == 0):
+        raise NativeError("route_weights must be fp32 and not empty")
+    two_f = 2 * width
+    dscore = torch.empty(rows, dtype=torch.float32, device=device)
+    gq = gs = gb = a_s = None
+    if quantized:
+        gq = torch.empty((rows, two_f), dtype=FP8, device=device)
+        gs = _scale_buffer(rows, two_f // 128, device)
+    if rounded:
+        gb = torch.empty((rows, two_f), dtype=torch.bfloat16, device=device)
+    if scaled_activation:
+        a_s = torch.empty((rows, width), dtype=torch.bfloat16, device=device)
+    if rows:
+        check(
+            lib.b200moe_dswiglu_saved8(
+                codes.data_ptr(), codes.stride(0), code_scales.data_ptr(), code_scales.stride(0),
+                code_scales.stride(1), r.data_ptr(), r.stride(0), weights.data_ptr(), weights.numel(),
+                order.data_ptr(), rows, width, dscore.data_ptr(), _ptr(gq), two_f, _ptr(gs),
+                0 if gs is None else gs.stride(0), 0 if gs is None else gs.stride(1), _ptr(gb), two_f, _ptr(a_s),
+                width, 0.0 if limit is None else float(limit), 0 if limit is None else 1,
+                status_block(device).data_ptr(), _stream(),
+            ),
+            "dswiglu_saved8",
+        )
+        _count()
+    return dscore, gq, gs, gb, a_s
+
+
 @_on_tensor_device
 def quantize_blocks(weight, *, out=None):
     """(data E4M3 [E,out,in], scale fp32 [E, ceil(out/128), ceil(in/128)]) of a bf16 or
@@ -945,12 +1063,13 @@ def whole_layer(x, w13, w2, experts, top_k) -> bool:
 
 @_on_tensor_device
 def forward_fp8(x, residual, logits, w13, w2, *, top_k, mode, bias=None, n_group=1, topk_group=1, routed_scaling=1.0,
-                limit=None):
+                limit=None, save8=False):
     """The forward pass behind the router GEMM as one host call: `(output, aux, counts,
     probability_sum, route_weights, route_ids, order, offsets, slots, h13)`, with the statistics of
     one sequence. The kernels and results of `route_topk`, `sort_assignments`,
     `quantize_rows_scatter`, `grouped_gemm_fp8`, `swiglu_quantize`, `combine` and
-    `routing_probability_sum` called in that order; for operands `whole_layer` accepts."""
+    `routing_probability_sum` called in that order; for operands `whole_layer` accepts. With `save8` the last
+    entry is h13 in 8 bits, `(codes, code_scales)` as `swiglu_save8` keeps it."""
     (w13_data, w13_scale), (w2_data, w2_scale) = w13, w2
     device = _need_cuda(x, residual, logits, w13_data, w13_scale, w2_data, w2_scale, bias)
     tokens, width = x.shape
@@ -975,9 +1094,15 @@ def forward_fp8(x, residual, logits, w13, w2, *, top_k, mode, bias=None, n_group
         weights.data_ptr(), ids.data_ptr(), order.data_ptr(), offsets.data_ptr(), slots.data_ptr(), counts.data_ptr(),
         h13.data_ptr(), output.data_ptr(), aux.data_ptr(), probability_sum.data_ptr(), x_q.data_ptr(),
         act_q.data_ptr(), expert_rows.data_ptr(), workspace.data_ptr(), status_block(device).data_ptr())
-    check(lib.b200moe_forward_fp8(ctypes.byref(args), _stream()), "forward_fp8")
+    saved = h13
+    if save8:
+        saved = new(torch.int8, rows, 2 * inner), new(torch.float32, rows, _saved_blocks(inner))
+        check(lib.b200moe_forward_fp8_save8(ctypes.byref(args), saved[0].data_ptr(), saved[1].data_ptr(), _stream()),
+              "forward_fp8_save8")
+    else:
+        check(lib.b200moe_forward_fp8(ctypes.byref(args), _stream()), "forward_fp8")
     _count(11 if rows > 4096 else 9)
-    return output, aux, counts, probability_sum, weights, ids, order, offsets, slots, h13
+    return output, aux, counts, probability_sum, weights, ids, order, offsets, slots, saved
 
 
 @_on_tensor_device
@@ -987,10 +1112,12 @@ def backward_fp8(grad_output, grad_aux, grad_probability_sum, x, w13, w2, logits
     """The backward pass up to the router as one host call: `(grad_x, grad_logits, high, low,
     grad_w13, grad_w2)`. `grad_x` lacks the router's share, `high + low` is `grad_logits` as two bf16
     pieces, a weight gradient nobody needs is None and is not computed. One buffer holds dy, x and
-    the input gradient's rows in turn. For operands `whole_layer` accepts."""
+    the input gradient's rows in turn. `h13` is the bf16 tensor or `(codes, code_scales)`. For operands
+    `whole_layer` accepts."""
     (w13_data, w13_scale), (w2_data, w2_scale) = w13, w2
+    saved8 = not isinstance(h13, torch.Tensor)
     device = _need_cuda(grad_output, grad_aux, grad_probability_sum, x, w13_data, w13_scale, w2_data, w2_scale, logits,
-                        route_weights, route_ids, order, offsets, slots, h13)
+                        route_weights, route_ids, order, offsets, slots, *(h13 if saved8 else (h13,)))
     tokens, width = x.shape
     experts, inner, top_k = logits.shape[1], w2_data.shape[2], route_ids.shape[1]
     rows = tokens * top_k
@@ -1010,10 +1137,14 @@ def backward_fp8(grad_output, grad_aux, grad_probability_sum, x, w13, w2, logits
         1 if weight_grad_dtype == torch.float32 else 0, 0.0 if limit is None else limit, grad_output.data_ptr(),
         _ptr(grad_aux), _ptr(grad_probability_sum), x.data_ptr(), w13_data.data_ptr(), w13_scale.data_ptr(),
         w2_data.data_ptr(), w2_scale.data_ptr(), logits.data_ptr(), route_weights.data_ptr(), route_ids.data_ptr(),
-        order.data_ptr(), offsets.data_ptr(), slots.data_ptr(), h13.data_ptr(), grad_x.data_ptr(),
+        order.data_ptr(), offsets.data_ptr(), slots.data_ptr(), None if saved8 else h13.data_ptr(), grad_x.data_ptr(),
         grad_logits.data_ptr(), high.data_ptr(), low.data_ptr(), _ptr(grad_w13), _ptr(grad_w2), dy_q.data_ptr(),
         row_buffer.data_ptr(), r.data_ptr(), gh_q.data_ptr(), _ptr(gh), workspace.data_ptr(),
         status_block(device).data_ptr())
-    check(lib.b200moe_backward_fp8(ctypes.byref(args), _stream()), "backward_fp8")
+    if saved8:
+        check(lib.b200moe_backward_fp8_saved8(ctypes.byref(args), h13[0].data_ptr(), h13[1].data_ptr(), _stream()),
+              "backward_fp8_saved8")
+    else:
+        check(lib.b200moe_backward_fp8(ctypes.byref(args), _stream()), "backward_fp8")
     _count(7 + (1 if need_w2 else 0) + (2 if need_w13 else 0) + (1 if grad_aux is not None else 0))
     return grad_x, grad_logits, high, low, grad_w13, grad_w2

@@ -56,6 +56,28 @@ def set_weight_gradient_operands(kind: str) -> str:
     return previous
 
 
+# What the routed layer and the shared expert keep of the pre-activation h13 between forward and backward: the
+# bf16 rows, or int8 codes in half the bytes (`ops.swiglu_save8`; the gradients are then those at the kept
+# values, within 1/254 of a 128-column block's largest magnitude). Read when a forward pass runs that can be
+# differentiated; the backward pass takes what its forward pass kept.
+SAVED_ACTIVATIONS = os.environ.get("B200MOE_SAVED_ACTIVATIONS", "bf16")
+
+
+def set_saved_activations(kind: str) -> str:
+    """`"bf16"` (default) or `"int8"`; returns the previous setting."""
+    global SAVED_ACTIVATIONS
+    if kind not in layer.SAVED_FORMS:
+        raise ValueError("saved activations are 'bf16' or 'int8'")
+    previous, SAVED_ACTIVATIONS = SAVED_ACTIVATIONS, kind
+    return previous
+
+
+def _saves_int8() -> bool:
+    if SAVED_ACTIVATIONS not in layer.SAVED_FORMS:
+        raise ValueError(f"saved activations are 'bf16' or 'int8', not {SAVED_ACTIVATIONS!r}")
+    return SAVED_ACTIVATIONS == "int8" and torch.is_grad_enabled()
+
+
 # ----------------------------------------------------------------- the reference's contexts
 def _context_weight_gradient_dtype():
     """The reference's `weight_gradients_at(...)` context, when the reference is present."""
@@ -159,6 +181,8 @@ class _DequantizedCopy(torch.autograd.Function):
 # ------------------------------------------------------------------ the operator pair
 _ELEVEN = tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor,
                 torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor]
+_TWELVE = tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor,
+                torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor]
 _FIVE = tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor]
 
 
@@ -181,6 +205,13 @@ def moe_fwd(h2: torch.Tensor, residual: torch.Tensor, router_weight: torch.Tenso
     slots, h13)`; `w13_experts` / `w2_experts` are the E4M3 data, `weight_components` their
     scales. `router_bias` with no elements means none."""
     del weight_grad_dtype
+    return _run_forward(h2, residual, router_weight, w13_experts, w2_experts, router_bias, top_k, routing_mode,
+                        n_group, topk_group, routed_scaling, lengths, weight_precision, swiglu_limit,
+                        weight_components, "bf16")
+
+
+def _run_forward(h2, residual, router_weight, w13_experts, w2_experts, router_bias, top_k, routing_mode, n_group,
+                 topk_group, routed_scaling, lengths, weight_precision, swiglu_limit, weight_components, saved):
     if weight_precision not in ROUTE_WEIGHT_PRECISIONS:
         raise ValueError(f"unsupported route-weight precision {weight_precision!r}")
     w13, w2 = _with_scales(w13_experts, w2_experts, weight_components)
@@ -188,7 +219,22 @@ def moe_fwd(h2: torch.Tensor, residual: torch.Tensor, router_weight: torch.Tenso
         return layer.forward_routed(
             h2, residual, router_weight, w13, w2, top_k=top_k, routing_mode=routing_mode,
             router_bias=None if router_bias.numel() == 0 else router_bias, n_group=n_group,
-            topk_group=topk_group, routed_scaling=routed_scaling, lengths=lengths, swiglu_limit=swiglu_limit)
+            topk_group=topk_group, routed_scaling=routed_scaling, lengths=lengths, swiglu_limit=swiglu_limit,
+            saved=saved)
+
+
+@torch.library.custom_op("b200moe::moe_save8_fwd", mutates_args=())
+def moe_save8_fwd(h2: torch.Tensor, residual: torch.Tensor, router_weight: torch.Tensor, w13_experts: torch.Tensor,
+                  w2_experts: torch.Tensor, router_bias: torch.Tensor, top_k: int, routing_mode: str, n_group: int,
+                  topk_group: int, routed_scaling: float, lengths: list[int], weight_precision: str,
+                  weight_grad_dtype: torch.dtype | None, swiglu_limit: float | None,
+                  weight_components: list[torch.Tensor]) -> _TWELVE:
+    """`moe_fwd` whose last result, h13, is kept in 8 bits: `(..., slots, codes, code_scales)`."""
+    del weight_grad_dtype
+    *results, kept = _run_forward(h2, residual, router_weight, w13_experts, w2_experts, router_bias, top_k,
+                                  routing_mode, n_group, topk_group, routed_scaling, lengths, weight_precision,
+                                  swiglu_limit, weight_components, "int8")
+    return (*results, *kept)
 
 
 @moe_fwd.register_fake
@@ -207,6 +253,14 @@ def _moe_fwd_fake(h2, residual, router_weight, w13_experts, w2_experts, router_b
         new((experts + 1,), torch.int32), new((rows, int(top_k)), torch.int32),
         new((assignments, w13_experts.shape[1]), h2.dtype),
     )
+
+
+@moe_save8_fwd.register_fake
+def _moe_save8_fwd_fake(h2, residual, router_weight, w13_experts, w2_experts, *rest):
+    *results, h13 = _moe_fwd_fake(h2, residual, router_weight, w13_experts, w2_experts, *rest)
+    rows, inner = h13.shape[0], w2_experts.shape[2]
+    return (*results, h13.new_empty(h13.shape, dtype=torch.int8),
+            h13.new_empty((rows, 2 * ((inner + 127) // 128)), dtype=torch.float32))
 
 
 def _given(cotangent):
@@ -228,6 +282,29 @@ def moe_bwd(grad_output: torch.Tensor, grad_aux: torch.Tensor, grad_probability_
     """`(grad_h2, grad_residual, grad_router, grad_w13, grad_w2)`; a gradient whose `need_*`
     flag is false is an empty placeholder and its GEMM is not launched. `grad_aux` and
     `grad_probability_sum` without elements mean none."""
+    return _run_backward(grad_output, grad_aux, grad_probability_sum, h2, router_weight, w13_experts, w2_experts, logits,
+                         route_weights, route_ids, order, offsets, slots, h13, top_k, routing_mode, lengths,
+                         weight_grad_dtype, swiglu_limit, need_router, need_w13, need_w2, weight_components)
+
+
+@torch.library.custom_op("b200moe::moe_saved8_bwd", mutates_args=())
+def moe_saved8_bwd(grad_output: torch.Tensor, grad_aux: torch.Tensor, grad_probability_sum: torch.Tensor,
+                   h2: torch.Tensor, router_weight: torch.Tensor, w13_experts: torch.Tensor,
+                   w2_experts: torch.Tensor, logits: torch.Tensor, route_weights: torch.Tensor,
+                   route_ids: torch.Tensor, order: torch.Tensor, offsets: torch.Tensor, slots: torch.Tensor,
+                   codes: torch.Tensor, code_scales: torch.Tensor, top_k: int, routing_mode: str,
+                   lengths: list[int], weight_grad_dtype: torch.dtype | None, swiglu_limit: float | None,
+                   need_router: bool, need_w13: bool, need_w2: bool,
+                   weight_components: list[torch.Tensor]) -> _FIVE:
+    """`moe_bwd` from what `moe_save8_fwd` kept."""
+    return _run_backward(grad_output, grad_aux, grad_probability_sum, h2, router_weight, w13_experts, w2_experts, logits,
+                         route_weights, route_ids, order, offsets, slots, (codes, code_scales), top_k, routing_mode,
+                         lengths, weight_grad_dtype, swiglu_limit, need_router, need_w13, need_w2, weight_components)
+
+
+def _run_backward(grad_output, grad_aux, grad_probability_sum, h2, router_weight, w13_experts, w2_experts, logits,
+                  route_weights, route_ids, order, offsets, slots, h13, top_k, routing_mode, lengths,
+                  weight_grad_dtype, swiglu_limit, need_router, need_w13, need_w2, weight_components):
     w13, w2 = _with_scales(w13_experts, w2_experts, weight_components)
     wdtype = _logical_dtype(weight_grad_dtype, torch.bfloat16)
     with torch.cuda.device(h2.device):
@@ -253,6 +330,11 @@ def _moe_bwd_fake(grad_output, grad_aux, grad_probability_sum, h2, router_weight
         new(tuple(w13_experts.shape), wdtype) if need_w13 else new((0,), wdtype),
         new(tuple(w2_experts.shape), wdtype) if need_w2 else new((0,), wdtype),
     )
+
+
+@moe_saved8_bwd.register_fake
+def _moe_saved8_bwd_fake(*args):
+    return _moe_bwd_fake(*args[:13], None, *args[15:])
 
 
 def _logical_flops(h2, router_weight, w13_experts, w2_experts, top_k, forward):
@@ -290,21 +372,32 @@ def _moe_bwd_flops(grad_output, grad_aux, grad_probability_sum, h2, router_weigh
     return _logical_flops(h2, router_weight, w13_experts, w2_experts, top_k, False)
 
 
+@register_flop_formula(torch.ops.b200moe.moe_save8_fwd, get_raw=True)
+def _moe_save8_fwd_flops(*args, out_val=None, **_kwargs):
+    return _moe_fwd_flops(*args)
+
+
+@register_flop_formula(torch.ops.b200moe.moe_saved8_bwd, get_raw=True)
+def _moe_saved8_bwd_flops(*args, out_val=None, **_kwargs):
+    return _moe_bwd_flops(*args[:14], *args[15:])
+
+
 def _setup_context(ctx, inputs, output):
     (h2, _residual, router_weight, w13_experts, w2_experts, _bias, top_k, routing_mode, _n_group, _topk_group,
      _scaling, lengths, _precision, weight_grad_dtype, swiglu_limit, weight_components) = inputs
-    (_out, _aux, counts, _psum, logits, route_weights, route_ids, order, offsets, slots, h13) = output
+    (_out, _aux, counts, _psum, logits, route_weights, route_ids, order, offsets, slots, *kept) = output
     ctx.save_for_backward(h2, router_weight, w13_experts, w2_experts, logits, route_weights, route_ids, order,
-                          offsets, slots, h13, *weight_components)
+                          offsets, slots, *kept, *weight_components)
     ctx.top_k, ctx.routing_mode, ctx.lengths = int(top_k), routing_mode, list(lengths)
     ctx.weight_grad_dtype, ctx.swiglu_limit = weight_grad_dtype, swiglu_limit
     # the gradient of a container goes out at its logical dtype unless the context names one
     ctx.logical = (w13_experts.dtype if w13_experts.dtype != torch.float8_e4m3fn else torch.bfloat16)
-    ctx.mark_non_differentiable(counts, logits, route_weights, route_ids, order, offsets, slots, h13)
+    ctx.mark_non_differentiable(counts, logits, route_weights, route_ids, order, offsets, slots, *kept)
     # an output without a cotangent arrives as None, not as a tensor of zeros: those of h13 alone
     # were a pass over [rows, 2F] bf16 in every backward
     ctx.set_materialize_grads(False)
     ctx.components = len(weight_components)
+    ctx.backward_operator = moe_bwd if len(kept) == 1 else moe_saved8_bwd
 
 
 def _requested(gradient, needed):
@@ -313,7 +406,8 @@ def _requested(gradient, needed):
 
 def _autograd_backward(ctx, grad_output, grad_aux, _g_counts, grad_probability_sum, *_metadata_grads):
     saved = ctx.saved_tensors
-    tensors, components = saved[:11], list(saved[11:])
+    end = len(saved) - ctx.components
+    tensors, components = saved[:end], list(saved[end:])
     h2, router_weight = tensors[0], tensors[1]
     if grad_output is None:
         grad_output = torch.zeros_like(h2)
@@ -328,7 +422,7 @@ def _autograd_backward(ctx, grad_output, grad_aux, _g_counts, grad_probability_s
     wdtype = ctx.weight_grad_dtype
     if wdtype is None and ctx.logical != torch.bfloat16:
         wdtype = ctx.logical
-    grad_h2, grad_residual, grad_router, grad_w13, grad_w2 = moe_bwd(
+    grad_h2, grad_residual, grad_router, grad_w13, grad_w2 = ctx.backward_operator(
         grad_output, grad_aux, grad_probability_sum, *tensors, ctx.top_k, ctx.routing_mode, ctx.lengths,
         wdtype, ctx.swiglu_limit, bool(need[2]), bool(need[3]), bool(need[4]), components)
     if ctx.weight_grad_dtype is None and need[2] and grad_router.dtype != router_weight.dtype:
@@ -339,6 +433,7 @@ def _autograd_backward(ctx, grad_output, grad_aux, _g_counts, grad_probability_s
 
 
 moe_fwd.register_autograd(_autograd_backward, setup_context=_setup_context)
+moe_save8_fwd.register_autograd(_autograd_backward, setup_context=_setup_context)
 
 
 # --------------------------------------------------------------- SwiGLU of the shared expert
@@ -403,8 +498,70 @@ def _swiglu_bwd_flops(h13, grad_act, limit, *_rest, out_val=None, **_kwargs):
     return 10 * (h13.numel() // 2)
 
 
+@torch.library.custom_op("b200moe::swiglu_save8", mutates_args=())
+def swiglu_save8(h13: torch.Tensor, limit: float | None) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """`swiglu` that keeps `h13` in 8 bits for its backward: `(act, codes [rows, 2F], code_scales)`."""
+    flat = h13.reshape(-1, h13.shape[-1])
+    if flat.stride(-1) != 1:
+        flat = flat.contiguous()
+    _, _, act, (codes, scales) = kernels.swiglu_save8(flat, limit=limit, quantized=False, rounded=True)
+    return act.reshape(*h13.shape[:-1], h13.shape[-1] // 2), codes, scales
+
+
+@swiglu_save8.register_fake
+def _swiglu_save8_fake(h13, limit):
+    rows, width = h13.numel() // h13.shape[-1], h13.shape[-1]
+    return (_swiglu_fake(h13, limit), h13.new_empty((rows, width), dtype=torch.int8),
+            h13.new_empty((rows, 2 * ((width // 2 + 127) // 128)), dtype=torch.float32))
+
+
+@torch.library.custom_op("b200moe::swiglu_saved8_bwd", mutates_args=())
+def swiglu_saved8_bwd(codes: torch.Tensor, code_scales: torch.Tensor, grad_act: torch.Tensor,
+                      limit: float | None) -> torch.Tensor:
+    """Gradient of `swiglu_save8` for its input, from what it kept (`grad_act [..., F]`)."""
+    grad = grad_act.reshape(-1, grad_act.shape[-1])
+    if grad.stride(-1) != 1:
+        grad = grad.contiguous()
+    rows = codes.shape[0]
+    ones = torch.ones(rows, dtype=torch.float32, device=codes.device)
+    identity = torch.arange(rows, dtype=torch.int32, device=codes.device)
+    _, _, _, grad_h13, _ = kernels.dswiglu_saved8((codes, code_scales), grad, ones, identity, limit=limit,
+                                                  quantized=False, rounded=True)
+    return grad_h13.reshape(*grad_act.shape[:-1], codes.shape[1])
+
+
+@swiglu_saved8_bwd.register_fake
+def _swiglu_saved8_bwd_fake(codes, code_scales, grad_act, limit):
+    return grad_act.new_empty((*grad_act.shape[:-1], codes.shape[1]))
+
+
+def _swiglu_save8_setup(ctx, inputs, output):
+    ctx.save_for_backward(*output[1:])
+    ctx.limit = inputs[1]
+    ctx.mark_non_differentiable(*output[1:])
+    ctx.set_materialize_grads(False)
+
+
+def _swiglu_save8_backward(ctx, grad_act, *_kept):
+    codes, scales = ctx.saved_tensors
+    return None if grad_act is None else swiglu_saved8_bwd(codes, scales, grad_act.contiguous(), ctx.limit), None
+
+
+swiglu_save8.register_autograd(_swiglu_save8_backward, setup_context=_swiglu_save8_setup)
+
+
+@register_flop_formula(torch.ops.b200moe.swiglu_save8, get_raw=True)
+def _swiglu_save8_flops(h13, limit, *_rest, out_val=None, **_kwargs):
+    return 5 * (h13.numel() // 2)
+
+
+@register_flop_formula(torch.ops.b200moe.swiglu_saved8_bwd, get_raw=True)
+def _swiglu_saved8_bwd_flops(codes, code_scales, grad_act, limit, *_rest, out_val=None, **_kwargs):
+    return 10 * (codes.numel() // 2)
+
+
 # ------------------------------------------------------------- containers at the boundary
-_CONTAINER_OPERATORS: list = [moe_fwd, moe_bwd]
+_CONTAINER_OPERATORS: list = [moe_fwd, moe_bwd, moe_save8_fwd, moe_saved8_bwd]
 _DISPATCH_REGISTERED: set = set()
 
 
@@ -468,7 +625,8 @@ def shared_expert(h2, shared_w13, shared_w2, shared_gate_weight=None, shared_mod
     ordinary differentiable graph: bf16 library GEMMs, as the reference computes it
     (`src/mlops/moe.py:12-37`; it never quantises the shared expert), around this library's
     SwiGLU operator."""
-    act = swiglu(torch.nn.functional.linear(h2, shared_w13), swiglu_limit)
+    h13 = torch.nn.functional.linear(h2, shared_w13)
+    act = swiglu_save8(h13, swiglu_limit)[0] if _saves_int8() else swiglu(h13, swiglu_limit)
     shared = torch.nn.functional.linear(act, shared_w2)
     if shared_mode == "sigmoid":
         gate = torch.sigmoid(torch.nn.functional.linear(h2, shared_gate_weight).float())
@@ -507,9 +665,10 @@ def apply(h2, residual, router_weight, w13_experts, w2_experts, *, top_k, routin
         # nothing to differentiate: what `_unwrap_containers` would hand on, without its detour
         components = [w13_experts._scale, w2_experts._scale]
         w13_experts, w2_experts = w13_experts._data, w2_experts._data
-    outputs = moe_fwd(h2, base, router_weight, w13_experts, w2_experts, bias, int(top_k), str(routing_mode),
-                      int(n_group), int(topk_group), float(routed_scaling), normalized,
-                      _context_route_weight_precision(), _context_weight_gradient_dtype(), limit, components)
+    operator = moe_save8_fwd if _saves_int8() else moe_fwd
+    outputs = operator(h2, base, router_weight, w13_experts, w2_experts, bias, int(top_k), str(routing_mode),
+                       int(n_group), int(topk_group), float(routed_scaling), normalized,
+                       _context_route_weight_precision(), _context_weight_gradient_dtype(), limit, components)
     return outputs[:4]
 
 
