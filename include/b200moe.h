@@ -567,6 +567,40 @@ int b200moe_backward_fp8_saved8(const b200moe_backward_args* args, const void* c
                                 void* stream);
 
 /*
+ * The whole layer for 1 to 64 tokens, as a serving loop calls it, without anything a backward pass would need:
+ * logits = x . bf16(router)^T, the routing of b200moe_route_topk, and
+ *   output[t] = residual[t] + sum_k w[t,k] W2[e] bf16(swiglu(W13[e] x[t]))  (+ the shared expert with weight 1)
+ * with fp32 sums, activations in bf16 and one rounding of the output.  Weights: E4M3 with fp32 scales per
+ * 128 x 128 block (both scale pointers; width and inner multiples of 128), or bf16 (both NULL; multiples of 8).
+ * experts <= 1024, top_k <= min(experts, 32), tokens <= 64.  Every matrix is dense; x and the weights are
+ * 16-byte aligned.  Results repeat bit for bit.
+ */
+typedef struct b200moe_decode_args {
+  long long tokens;
+  int width, inner, experts, top_k;
+  int mode, n_group, topk_group, limited;
+  int router_is_fp32, shared_inner;
+  float routed_scaling, limit;
+  const void* x;        /* bf16 [tokens, width] */
+  const void* residual; /* bf16 [tokens, width] */
+  const void* router;   /* fp32 or bf16 [experts, width]; multiplied as bf16 */
+  const float* bias;    /* fp32 [experts] or NULL */
+  const void* w13;      /* [experts, 2 inner, width], gate rows then up rows */
+  const float* w13_scale;
+  const void* w2; /* [experts, width, inner] */
+  const float* w2_scale;
+  const void* shared_w13; /* bf16 [2 shared_inner, width] and [width, shared_inner]; shared_inner 0: none */
+  const void* shared_w2;
+  float* route_weights; /* results: [tokens, top_k] */
+  int32_t* ids;         /* [tokens, top_k] */
+  void* output;         /* bf16 [tokens, width] */
+  void* workspace;      /* b200moe_decode_workspace_bytes, 256-byte aligned */
+} b200moe_decode_args;
+long long b200moe_decode_workspace_bytes(long long tokens, int width, int inner, int experts, int top_k,
+                                         int shared_inner);
+int b200moe_decode(const b200moe_decode_args* args, void* stream);
+
+/*
  * dst[slots[t * fanout + k], :] = src[t, :] (bf16 rows of `width`): b200moe_gather_rows with
  * gather = order, gather_div = fanout, from the token's side.  A slot outside [0, rows_out) is
  * reported and skipped.  fanout <= 32.

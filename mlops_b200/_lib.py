@@ -53,6 +53,16 @@ class BackwardArgs(ctypes.Structure):
             "grad_logits_low", "grad_w13", "grad_w2", "dy_q", "rows", "r", "gh_q", "gh", "workspace", "status")]
 
 
+class DecodeArgs(ctypes.Structure):
+    """`b200moe_decode_args`"""
+
+    _fields_ = [("tokens", LL)] + [(n, I) for n in (
+        "width", "inner", "experts", "top_k", "mode", "n_group", "topk_group", "limited", "router_is_fp32",
+        "shared_inner")] + [("routed_scaling", F), ("limit", F)] + [(n, P) for n in (
+            "x", "residual", "router", "bias", "w13", "w13_scale", "w2", "w2_scale", "shared_w13", "shared_w2",
+            "route_weights", "ids", "output", "workspace")]
+
+
 # name -> (restype, argtypes); one entry per declaration in include/b200moe.h
 SIGNATURES = {
     "b200moe_route_topk": (I, [P, LL, I, I, I, I, P, I, I, F, P, P, P]),
@@ -113,6 +123,8 @@ SIGNATURES = {
     "b200moe_backward_fp8": (I, [P, P]),
     "b200moe_forward_fp8_save8": (I, [P, P, P, P]),
     "b200moe_backward_fp8_saved8": (I, [P, P, P, P]),
+    "b200moe_decode_workspace_bytes": (LL, [LL, I, I, I, I, I]),
+    "b200moe_decode": (I, [P, P]),
     "b200moe_gather_scalar": (I, [P, LL, P, LL, P, P, P]),
 }
 

@@ -236,6 +236,37 @@ def forward_routed(
     return (output, aux, counts, probability_sum, logits, route_weights, route_ids, order, offsets, slots, h13)
 
 
+def forward_decode(
+    h2: torch.Tensor,
+    residual: torch.Tensor,
+    router_weight: torch.Tensor,
+    w13: torch.Tensor | tuple[torch.Tensor, torch.Tensor],
+    w2: torch.Tensor | tuple[torch.Tensor, torch.Tensor],
+    *,
+    top_k: int,
+    routing_mode: str,
+    router_bias: torch.Tensor | None = None,
+    n_group: int = 1,
+    topk_group: int = 1,
+    routed_scaling: float = 1.0,
+    swiglu_limit: float | None = None,
+    shared: tuple[torch.Tensor, torch.Tensor] | None = None,
+) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """The layer for 1 to 64 tokens of a serving loop: `(output, route_weights, route_ids)`, arguments as
+    `forward_routed` takes them. One host call that reads each needed weight once; nothing is kept for a
+    backward pass and no statistics are formed. Activations stay bf16 on block-FP8 weights too
+    (`forward_routed` quantises them to E4M3), so the output is the nearer of the two to the weights' exact product.
+    `shared = (w13 [2Fs, D], w2 [D, Fs])` (bf16) adds the always-on shared expert."""
+    with torch.no_grad():
+        rows = h2.reshape(-1, h2.shape[-1]).contiguous()
+        bias = None if router_bias is None or router_bias.numel() == 0 else router_bias
+        output, weights, ids = ops.moe_decode(
+            rows, residual.reshape(rows.shape).contiguous(), getattr(router_weight, "_data", router_weight), w13, w2,
+            top_k=top_k, mode=str(routing_mode), bias=bias, n_group=n_group, topk_group=topk_group,
+            routed_scaling=routed_scaling, limit=swiglu_limit, shared=shared)
+        return output.view(h2.shape), weights, ids
+
+
 def _swiglu(h13, save8, **kwargs):
     """SwiGLU and what is kept of its input: `(act_q, scales, act_bf16, kept)`."""
     if save8:

@@ -16,7 +16,7 @@ import os
 
 import torch
 
-from ._lib import BackwardArgs, ForwardArgs, NativeError, check, lib
+from ._lib import BackwardArgs, DecodeArgs, ForwardArgs, NativeError, check, lib
 
 ROUTING_MODES = {"topk_then_softmax": 0, "softmax_then_topk": 1, "sigmoid_noaux_tc": 2}
 FP8 = torch.float8_e4m3fn
@@ -1148,3 +1148,88 @@ def backward_fp8(grad_output, grad_aux, grad_probability_sum, x, w13, w2, logits
         check(lib.b200moe_backward_fp8(ctypes.byref(args), _stream()), "backward_fp8")
     _count(7 + (1 if need_w2 else 0) + (2 if need_w13 else 0) + (1 if grad_aux is not None else 0))
     return grad_x, grad_logits, high, low, grad_w13, grad_w2
+
+
+# ------------------------------------------------------------------ the layer for a few tokens
+DECODE_TOKENS = 64  # what `moe_decode` takes at most
+
+
+def _decode_weights(w13, w2):
+    """`(w13, w13_scale, w2, w2_scale)` of bf16 weights (scales None) or of (E4M3 data, block scales) pairs."""
+    if isinstance(w13, torch.Tensor):
+        if not isinstance(w2, torch.Tensor) or w13.dtype != torch.bfloat16 or w2.dtype != torch.bfloat16:
+            raise NativeError("expert weights are both bf16 tensors or both (E4M3 data, fp32 block scales)")
+        scales = (None, None)
+    else:
+        if isinstance(w2, torch.Tensor):
+            raise NativeError("expert weights are both bf16 tensors or both (E4M3 data, fp32 block scales)")
+        (w13, s13), (w2, s2) = w13, w2
+        if w13.dtype != FP8 or w2.dtype != FP8 or s13.dtype != torch.float32 or s2.dtype != torch.float32:
+            raise NativeError("expert weights are both bf16 tensors or both (E4M3 data, fp32 block scales)")
+        scales = (s13, s2)
+    if w13.dim() != 3 or w2.dim() != 3:
+        raise NativeError("expected w13 [E, 2F, D] and w2 [E, D, F]")
+    experts, width, inner = w2.shape
+    if w13.shape != (experts, 2 * inner, width):
+        raise NativeError("expected w13 [E, 2F, D] and w2 [E, D, F]")
+    step = 8 if scales[0] is None else 128
+    if width % step or inner % step or inner == 0 or width == 0:
+        raise NativeError(f"D and F must be multiples of {step}")
+    if scales[0] is not None and (scales[0].shape != (experts, inner // 64, width // 128)
+                                  or scales[1].shape != (experts, width // 128, inner // 128)):
+        raise NativeError("block scales must be [E, 2F / 128, D / 128] and [E, D / 128, F / 128]")
+    for t in (w13, w2, *scales):
+        if t is not None and not t.is_contiguous():
+            raise NativeError("weights and their scales must be contiguous")
+    return w13, scales[0], w2, scales[1]
+
+
+@_on_tensor_device
+def moe_decode(x, residual, router, w13, w2, *, top_k, mode, bias=None, n_group=1, topk_group=1, routed_scaling=1.0,
+               limit=None, shared=None):
+    """The whole layer for 1 to 64 tokens: `(output bf16 [T, D], route_weights fp32 [T, K], ids int32 [T, K])`
+    of bf16 `x`, `residual [T, D]`, the router `[E, D]` (fp32 or bf16; multiplied as bf16) and expert
+    weights `w13 [E, 2F, D]`, `w2 [E, D, F]`, bf16 or (E4M3 data, block scales). Activations stay bf16, every sum is
+    fp32, results repeat bit for bit. `shared = (w13 [2Fs, D], w2 [D, Fs])` adds the shared expert (bf16)."""
+    w13, s13, w2, s2 = _decode_weights(w13, w2)
+    shared13, shared2 = (None, None) if shared is None else shared
+    device = _need_cuda(x, residual, router, bias, w13, s13, w2, s2, shared13, shared2)
+    tokens, width = x.shape
+    experts, inner, top_k = w2.shape[0], w2.shape[2], int(top_k)
+    if tokens > DECODE_TOKENS:
+        raise NativeError(f"at most {DECODE_TOKENS} tokens: the grouped layer (forward_routed) takes more")
+    if not (dense(x, torch.bfloat16, tokens, w2.shape[1]) and dense(residual, torch.bfloat16, tokens, width)):
+        raise NativeError(f"x and residual must be contiguous bf16 [tokens, {w2.shape[1]}]")
+    if router.dtype not in (torch.float32, torch.bfloat16) or router.shape != (experts, width) \
+            or not router.is_contiguous():
+        raise NativeError(f"the router must be contiguous fp32 or bf16 [{experts}, {width}]")
+    if mode not in ROUTING_MODES:
+        raise NativeError(f"unsupported routing mode {mode!r}")
+    if experts > 1024 or not 0 < top_k <= min(experts, 32):
+        raise NativeError("supported sizes: experts <= 1024, 0 < top_k <= min(experts, 32)")
+    if bias is not None:
+        if bias.numel() != experts:
+            raise NativeError("router_bias has one entry per expert")
+        bias = bias.to(torch.float32).contiguous()
+    shared_inner = 0
+    if shared13 is not None:
+        shared_inner = shared2.shape[-1]
+        if not (dense(shared13, torch.bfloat16, 2 * shared_inner, width)
+                and dense(shared2, torch.bfloat16, width, shared_inner)) or shared_inner % 8 or shared_inner == 0:
+            raise NativeError("shared weights must be contiguous bf16 [2Fs, D] and [D, Fs], Fs a multiple of 8")
+    output = torch.empty_like(x)
+    weights = torch.empty((tokens, top_k), dtype=torch.float32, device=device)
+    ids = torch.empty((tokens, top_k), dtype=torch.int32, device=device)
+    if tokens == 0:
+        return output, weights, ids
+    workspace = torch.empty(lib.b200moe_decode_workspace_bytes(tokens, width, inner, experts, top_k, shared_inner),
+                            dtype=torch.uint8, device=device)
+    args = DecodeArgs(
+        tokens, width, inner, experts, top_k, ROUTING_MODES[mode], int(n_group), int(topk_group),
+        0 if limit is None else 1, 1 if router.dtype == torch.float32 else 0, shared_inner, float(routed_scaling),
+        0.0 if limit is None else float(limit), x.data_ptr(), residual.data_ptr(), router.data_ptr(), _ptr(bias),
+        w13.data_ptr(), _ptr(s13), w2.data_ptr(), _ptr(s2), _ptr(shared13), _ptr(shared2), weights.data_ptr(),
+        ids.data_ptr(), output.data_ptr(), workspace.data_ptr())
+    check(lib.b200moe_decode(ctypes.byref(args), _stream()), "moe_decode")
+    _count(4)
+    return output, weights, ids
