@@ -595,6 +595,7 @@ typedef struct b200moe_decode_args {
   int32_t* ids;         /* [tokens, top_k] */
   void* output;         /* bf16 [tokens, width] */
   void* workspace;      /* b200moe_decode_workspace_bytes, 256-byte aligned */
+  int32_t* status;
 } b200moe_decode_args;
 long long b200moe_decode_workspace_bytes(long long tokens, int width, int inner, int experts, int top_k,
                                          int shared_inner);

@@ -60,7 +60,7 @@ class DecodeArgs(ctypes.Structure):
         "width", "inner", "experts", "top_k", "mode", "n_group", "topk_group", "limited", "router_is_fp32",
         "shared_inner")] + [("routed_scaling", F), ("limit", F)] + [(n, P) for n in (
             "x", "residual", "router", "bias", "w13", "w13_scale", "w2", "w2_scale", "shared_w13", "shared_w2",
-            "route_weights", "ids", "output", "workspace")]
+            "route_weights", "ids", "output", "workspace", "status")]
 
 
 # name -> (restype, argtypes); one entry per declaration in include/b200moe.h

@@ -1,48 +1,103 @@
 // The routed layer for a few tokens (1 to 64), as a serving loop calls it: router logits, expert selection, up
 // product with SwiGLU, down product with the weighted sum, residual and shared expert.
 //
-//   logits = x . bf16(router)^T                          router_logits_kernel
+//   logits = x . bf16(router)^T                                          router_logits_kernel
 //   (weights, ids) = the routing of route.cu
-//   act[t,k] = bf16(silu(g) * u), [g | u] = x[t] . W13[e]^T          stream_kernel<UP>
-//   out[t] = residual[t] + sum_k w[t,k] act[t,k] . W2[e]^T (+ the shared expert's)   stream_kernel<DOWN>
+//   act[t,k] = bf16(silu(g) * u), [g | u] = x[t] . W13[e]^T              stream_kernel<UP>
+//   y[t,k] = act[t,k] . W2[e]^T                                          stream_kernel<DOWN>
+//   out[t] = residual[t] + sum_k w[t,k] y[t,k] (+ the shared expert's)   join_kernel
 //
 // Bound: HBM.  The weights of the experts that got a token are read once, 3 D F bytes each in E4M3, for one
 // or a few multiplications a byte; everything else is small.  So the two products are one stream of weight
-// rows through shared memory (16-byte asynchronous copies, several stages of 16 KB in flight per SM), cut evenly over
-// the SMs to the single row: with whole tiles of 64 columns eight experts of F = 768 would leave 52 of 148 SMs idle.
+// rows through shared memory (boxes of 128 bytes of K, several stages of 32 KB in flight per SM), and the rows of all experts
+// with tokens, one after the other, are cut evenly over the CTAs in groups of eight: with whole tiles of 64 columns
+// eight experts of F = 768 would leave 52 of 148 SMs idle.  Cutting the down product's output columns instead, which
+// needs no y, left a CTA 14 to 24 rows of each expert: the tokens' columns then weigh as much as the weights'.
 //
-// The weights are the A operand of mma.m16n8k16 (16 weight rows), the tokens the B operand (8 to a
-// tile).  Activations stay bf16: E4M3 weights are widened to bf16, which holds every E4M3 value, and the
-// 128 x 128 block scales are applied in fp32 to the sums of one 128-column block, so nothing is quantised.  tcgen05
-// has no product of E4M3 by bf16 and its tiles start at 64 rows; at one to eight tokens a weight row the
-// tensor rate is not what bounds this.  Sums are fp32; act is rounded to bf16 once, as the operand of the second product
-// (the grouped layer rounds it likewise), and the output once.  Every sum has a fixed order: no atomics.
+// The weights are the A operand of mma.sync.m16n8k16 (16 weight rows), the tokens the B operand (8 to a tile).
+// Against bf16 weights the tokens are bf16.  E4M3 weights are widened to f16, one instruction for two values, and a
+// token's block of 128 columns is f16 with a power of two per block that puts its largest value in [2^14, 2^15): every
+// bf16 value down to 2^-29 of the largest exactly, what is smaller within 2^-40 of it.  The 128 x 128 block scales and
+// the tokens' powers of two are applied in fp32 to the sums of one block.  (Widening to bf16 takes four
+// instructions for two values, 200 of the 356 issue slots an SM has per 2 KB of weights at full HBM rate;
+// m16n8k32 on E4M3 operands widens them inside, again for every tile: 22 cycles against 8 of m16n8k16.)
+//
+// tcgen05 is not used: it has no product of E4M3 by 16-bit values, its tiles start at 64 rows, and at one to eight tokens
+// a weight row the tensor rate is not what bounds this.  Sums are fp32; act is rounded to bf16 once, as the operand of the
+// second product (the grouped layer rounds it likewise), and the output once.  Every sum has a fixed order: no
+// atomics.
 #include "common.cuh"
 #include "host_util.h"
 #include "../../include/b200moe.h"
 
 namespace b200 {
 
-constexpr int kDecodeThreads = 256;
+constexpr int kDecodeThreads = 256;  // of the small kernels
 constexpr int kDecodeWarps = 8;
+constexpr int kMultiplyWarps = 16;    // of a stream
+constexpr int kFillWarps = 4;         // of a stream: they keep its stages full
+constexpr int kStreamThreads = 32 * (kMultiplyWarps + kFillWarps);
 constexpr int kMaxTokens = 64;
-constexpr int kSlab = 2048;               // 16 weight rows x 128 bytes of K
-constexpr int kStageA = 8 * kSlab;        // a stage holds eight slabs: row tiles x K blocks
-constexpr int kStageScales = 8 * 16 * 4;  // one scale per row of a slab
+constexpr int kSlab = 2048;           // 16 weight rows x 128 bytes of K
+constexpr int kStageSlabs = 16;       // of a stage: row tiles x K blocks, one to a multiplying warp
+constexpr int kStageA = kStageSlabs * kSlab;
+constexpr int kTokenBytes = 256;      // a token's 128 columns beside an E4M3 block, and
+constexpr int kTokenPitchBf16 = 192;  // its 64 beside a bf16 block: rows start in different banks
+constexpr int kStageScales = 2 * kStageSlabs;  // of the weights: each slab's first and other eight rows
+constexpr int kMaxStages = 8;
+constexpr int kPassTokens = 32;  // of one expert that a pass over its weights takes; rarely has an expert more
 
 __device__ __forceinline__ void copy16(void* dst, const void* src, bool read) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(dst)), "l"(src), "r"(read ? 16 : 0)
                : "memory");
 }
+// One arrival on `bar` (which counts it) when this thread's copies so far have landed.
+__device__ __forceinline__ void copies_arrive(uint64_t* bar) {
+  asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
+}
+
 __device__ __forceinline__ void copy4(void* dst, const void* src) {
   asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(smem_u32(dst)), "l"(src) : "memory");
 }
-__device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int LEFT>
-__device__ __forceinline__ void copies_wait() {
-  asm volatile("cp.async.wait_group %0;" ::"n"(LEFT) : "memory");
+
+// mbar_wait for a whole warp whose poll sleeps up to 100 us at a time: what waits here waits for HBM, and polling took a third
+// of the SM's issue slots.
+__device__ __forceinline__ bool wait_stage(uint64_t* bar, uint32_t parity, volatile int* abort_flag, int* status,
+                                           int where) {
+  int ok = 1;
+  if ((threadIdx.x & 31) == 0) {
+    const long long start = clock64();
+    for (;;) {
+      uint32_t done;
+      asm volatile(
+          "{\n\t.reg .pred P;\n\t"
+          "mbarrier.try_wait.parity.shared::cta.b64 P, [%1], %2, 100000;\n\t"
+          "selp.u32 %0, 1, 0, P;\n\t}"
+          : "=r"(done)
+          : "r"(smem_u32(bar)), "r"(parity)
+          : "memory");
+      if (done) break;
+      const bool late = clock64() - start > B200_WAIT_LIMIT_CYCLES;
+      if (*abort_flag || late) {
+        if (late) {
+          *abort_flag = 1;
+          report_error(status, ERR_WAIT_TIMEOUT, where, (int)parity);
+        }
+        ok = 0;
+        break;
+      }
+    }
+  }
+  return __shfl_sync(0xffffffffu, ok, 0) != 0;
 }
 
+__device__ __forceinline__ void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                        uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
 __device__ __forceinline__ void mma_bf16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
                                          uint32_t b1) {
   asm volatile(
@@ -51,14 +106,29 @@ __device__ __forceinline__ void mma_bf16(float (&c)[4], uint32_t a0, uint32_t a1
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
-// Two E4M3 values as bf16 (through f16, exact both ways).
-__device__ __forceinline__ uint32_t widen2(uint32_t pair) {
-  const __half2 h = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(pair & 0xffffu), __NV_E4M3);
-  const float2 f = __half22float2(h);
-  return pack_bf16x2(f.x, f.y);
+// Four E4M3 values as two pairs of f16 (exact).
+__device__ __forceinline__ void widen(uint32_t w, uint32_t& first, uint32_t& second) {
+  asm("{\n\t.reg .b16 l, h;\n\tmov.b32 {l, h}, %2;\n\t"
+      "cvt.rn.f16x2.e4m3x2 %0, l;\n\tcvt.rn.f16x2.e4m3x2 %1, h;\n\t}"
+      : "=r"(first), "=r"(second)
+      : "r"(w));
 }
 
-__device__ __forceinline__ uint32_t word(const uint4& v, int i) { return i == 0 ? v.x : i == 1 ? v.y : i == 2 ? v.z : v.w; }
+// A warp scales 128 bf16 values, four to a lane, to f16 by the block's power of two (see the top), which it returns.
+__device__ __forceinline__ float scale_block(const uint2& raw, uint2& out) {
+  uint32_t m = __vmaxu2(raw.x & 0x7fff7fffu, raw.y & 0x7fff7fffu);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) m = __vmaxu2(m, __shfl_xor_sync(0xffffffffu, m, o));
+  // exponent of the largest, kept where both powers of two are normal numbers
+  const int e = min(max((int)(max(m & 0xffffu, m >> 16) >> 7), 27), 254);
+  const float inverse = __int_as_float((268 - e) << 23);  // largest / s in [2^14, 2^15)
+  const __nv_bfloat162* pairs = reinterpret_cast<const __nv_bfloat162*>(&raw);
+  const float2 a = __bfloat1622float2(pairs[0]), b = __bfloat1622float2(pairs[1]);
+  const __half2 first = __floats2half2_rn(a.x * inverse, a.y * inverse);
+  const __half2 second = __floats2half2_rn(b.x * inverse, b.y * inverse);
+  out = make_uint2(*reinterpret_cast<const uint32_t*>(&first), *reinterpret_cast<const uint32_t*>(&second));
+  return __int_as_float((e - 14) << 23);
+}
 
 // ---------------------------------------------------------------------------------------------
 // Router logits, fp32 [T, E]: 16 experts per cluster of eight CTAs, which split the hidden width between
@@ -89,11 +159,23 @@ __device__ __forceinline__ void load_router(const W* row, int k, int width, bool
 template <typename W, int NT>
 __global__ void __launch_bounds__(kDecodeThreads)
 router_logits_kernel(const __nv_bfloat16* __restrict__ x, const W* __restrict__ router, int T, int E, int width,
-                     float* __restrict__ logits) {
+                     float* __restrict__ logits, uint8_t* __restrict__ x16, float* __restrict__ x16_scale) {
   __shared__ float partial[kDecodeWarps][NT * 8][16];
   __shared__ float sums[NT * 8][16];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   const int rank = (int)cluster_ctarank();
+  const int routers = (E + 15) / 16 * kRouterCluster;
+  if ((int)blockIdx.x >= routers) {  // the clusters behind the router's scale the tokens for the E4M3 products
+    const int blocks = width / 128;
+    const int warps = ((int)gridDim.x - routers) * kDecodeWarps;
+    for (int i = ((int)blockIdx.x - routers) * kDecodeWarps + warp; i < T * blocks; i += warps) {
+      uint2 scaled;
+      const float scale = scale_block(reinterpret_cast<const uint2*>(x)[(long long)i * 32 + lane], scaled);
+      reinterpret_cast<uint2*>(x16)[(long long)i * 32 + lane] = scaled;
+      if (lane == 0) x16_scale[i] = scale;
+    }
+    return;
+  }
   const int e0 = (blockIdx.x / kRouterCluster) * 16;
   const W* lo = router + (long long)(e0 + g) * width;
   const W* hi = lo + 8LL * width;
@@ -159,32 +241,42 @@ struct DecodeParams {
   const uint8_t *w13, *w2;  // E4M3 or bf16
   const float *w13_scale, *w2_scale;
   const uint8_t *shared_w13, *shared_w2;  // bf16, or null
+  const uint8_t* x16;                     // x against E4M3 weights: [T, D / 128, 256]
+  const float* x16_scale;               // [T, D / 128]
   __nv_bfloat16* act;                     // [T * K, F] in expert order
   __nv_bfloat16* act_shared;              // [T, shared_inner]
+  uint8_t* act16;                         // act against E4M3 weights: [T * K, F / 128, 256]
+  float* act16_scale;                     // [T * K, F / 128]
+  float* y;                               // [T * K (+ T), D] in expert order, the shared expert's last
+  int* row_of;                            // [T * K] row of each assignment
   __nv_bfloat16* out;
   int T, D, F, E, K, shared_inner;
   int fp8, limited;
   float limit;
-  int b_rows;  // capacity of a stage's B part, in rows of one K block
+  int b_rows;  // capacity of a stage's token part, in rows of one K block
+  int* status;
+};
+
+// Weight rows as [experts * rows, K], read in boxes of `tall` (UP: 128, DOWN: 256) or 8 rows x 128 bytes.
+struct DecodeMaps {
+  CUtensorMap tall, flat, shared_tall, shared_flat;
 };
 
 // Where things are in shared memory behind the stages.
 struct Lists {
   int* begin;          // [experts with tokens + 1] first row of each
-  float* weights;      // [T * K] route weight of each row
   uint16_t* expert;    // [experts with tokens]
   uint8_t* tokens;     // [T * K]
   int* scratch;        // [E + 64]
   uint16_t* rank;      // [T * K]
   __host__ __device__ static int bytes(int T, int E, int K) {
     const int R = T * K, most = E < R ? E : R;
-    return 4 * (most + 1) + 4 * R + 4 * (E + 64) + 2 * (most + R) + R + 64;
+    return 4 * (most + 1) + 4 * (E + 64) + 2 * (most + R) + R + 64;
   }
   __device__ void place(uint8_t* base, int T, int E, int K) {
     const int R = T * K, most = E < R ? E : R;
     begin = reinterpret_cast<int*>(base);
-    weights = reinterpret_cast<float*>(begin + most + 1);
-    scratch = reinterpret_cast<int*>(weights + R);
+    scratch = begin + most + 1;
     expert = reinterpret_cast<uint16_t*>(scratch + E + 64);
     rank = expert + most;
     tokens = reinterpret_cast<uint8_t*>(rank + R);
@@ -192,12 +284,12 @@ struct Lists {
 };
 
 // Rows by expert, in token order inside one; returns the number of experts with tokens.
-__device__ __forceinline__ int build_lists(const Lists& l, const int* __restrict__ ids,
-                                           const float* __restrict__ route_weights, int T, int E, int K) {
+__device__ __forceinline__ int build_lists(const Lists& l, const int* __restrict__ ids, int T, int E, int K,
+                                           int* __restrict__ row_of) {
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, R = T * K;
   int* count = l.scratch;           // per expert: rows, then first row
   int* totals = l.scratch + E;      // per warp
-  for (int e = tid; e < E; e += kDecodeThreads) count[e] = 0;
+  for (int e = tid; e < E; e += kStreamThreads) count[e] = 0;
   __syncthreads();
   if (warp == 0) {
     for (int base = 0; base < R; base += 32) {
@@ -214,7 +306,7 @@ __device__ __forceinline__ int build_lists(const Lists& l, const int* __restrict
   }
   __syncthreads();
   // exclusive sums over the experts of (rows, experts with rows), packed in one word
-  const int per = (E + kDecodeThreads - 1) / kDecodeThreads;
+  const int per = (E + kStreamThreads - 1) / kStreamThreads;
   int mine = 0;
   for (int j = 0; j < per; ++j) {
     const int e = tid * per + j;
@@ -231,7 +323,7 @@ __device__ __forceinline__ int build_lists(const Lists& l, const int* __restrict
   int at = incl - mine;
   for (int w = 0; w < warp; ++w) at += totals[w];
   int active = 0;
-  for (int w = 0; w < kDecodeWarps; ++w) active += totals[w];
+  for (int w = 0; w < kStreamThreads / 32; ++w) active += totals[w];
   active >>= 16;
   for (int j = 0; j < per; ++j) {
     const int e = tid * per + j;
@@ -246,18 +338,18 @@ __device__ __forceinline__ int build_lists(const Lists& l, const int* __restrict
   }
   if (tid == 0) l.begin[active] = R;
   __syncthreads();
-  for (int i = tid; i < R; i += kDecodeThreads) {
+  for (int i = tid; i < R; i += kStreamThreads) {
     const int at_row = count[ids[i]] + l.rank[i];
-    l.weights[at_row] = route_weights[i];
+    if (row_of != nullptr) row_of[i] = at_row;
     l.tokens[at_row] = (uint8_t)(i / K);
   }
   __syncthreads();
   return active;
 }
 
-// A piece of the stream: consecutive output columns (UP: of the activation, gate and up rows alike; DOWN: of the
-// output) of one expert.  Its rows are cut into 1 << rt_log tiles of 16, the K blocks of a stage go to the
-// 1 << ks_log warps of each tile.
+// A piece of the stream: consecutive output columns of one expert (UP: of the activation, gate and up rows alike; DOWN:
+// of y), at most 128 or 256, and at most kPassTokens of its tokens.  Its rows are cut into 1 << rt_log tiles of 16; a stage has
+// 1 << ks_log K blocks of them.  Slab (K block << rt_log) + tile belongs to the warp of that number.
 struct Piece {
   int index;         // expert with tokens, or `active` for the shared expert
   int first, count;  // output columns
@@ -271,240 +363,254 @@ template <bool DOWN>
 struct Stream {
   const DecodeParams& p;
   const Lists& l;
-  int active;
-  int at, end;  // UP: flat activation columns of the experts with tokens, then the shared expert's; DOWN: output columns
-  int row_first, row_count, which;  // DOWN: current run of output columns, next expert
-  int step;
-  bool done;
+  const int active;
+  int at, end;  // flat output columns of the experts with tokens, then the shared expert's
+  int waiting;  // tokens of the current expert that need another pass over the same weights
   Piece piece;
 
-  __device__ Stream(const DecodeParams& params, const Lists& lists, int n_active) : p(params), l(lists), active(n_active) {
+  // The columns are cut between the CTAs in whole groups of eight, what a flat box of weights holds.
+  __device__ Stream(const DecodeParams& params, const Lists& lists, int n_active)
+      : p(params), l(lists), active(n_active), waiting(0) {
     const long long b = blockIdx.x, grid = gridDim.x;
-    if (DOWN) {
-      at = (int)(p.D * b / grid);
-      end = (int)(p.D * (b + 1) / grid);
-      row_first = at;
-      row_count = min(128, end - at);
-      which = 0;
-    } else {
-      const long long total = (long long)active * p.F + (long long)shared_weight() * p.shared_inner;
-      at = (int)(total * b / grid);
-      end = (int)(total * (b + 1) / grid);
-    }
-    done = false;
-    open();
+    const long long total = (long long)active * width() + (long long)shared_cost() * shared_width();
+    at = (int)(total / 8 * b / grid) * 8;
+    end = (int)(total / 8 * (b + 1) / grid) * 8;
   }
-  // a column of a bf16 shared expert costs twice what an E4M3 expert's does
-  __device__ int shared_weight() const { return p.fp8 ? 2 : 1; }
-  __device__ int shared_column(int flat) const { return (flat - active * p.F + shared_weight() - 1) / shared_weight(); }
+  __device__ int width() const { return DOWN ? p.D : p.F; }
+  __device__ int shared_width() const { return p.shared_inner == 0 ? 0 : DOWN ? p.D : p.shared_inner; }
+  // what a column of the shared expert (bf16) costs in columns of the others
+  __device__ int shared_cost() const {
+    const int bytes = p.fp8 ? 2 : 1;
+    return !DOWN ? bytes : min(max((p.shared_inner * bytes + p.F / 2) / p.F, 1), 64);
+  }
+  __device__ int shared_column(int flat) const {
+    const int group = shared_cost() * 8;
+    return (flat - active * width() + group - 1) / group * 8;
+  }
 
-  __device__ void open() {
-    step = 0;
-    if (DOWN) {
-      const int experts = active + (p.shared_inner > 0 ? 1 : 0);
-      if (which == experts) {
-        which = 0;
-        row_first += row_count;
-        row_count = min(128, end - row_first);
-      }
-      if (row_count <= 0) {
-        done = true;
-        return;
-      }
-      piece.index = which++;
-      piece.first = row_first;
-      piece.count = row_count;
-    } else {
-      for (;;) {
-        if (at >= end) {
-          done = true;
-          return;
-        }
-        if (at < active * p.F) {
-          piece.index = at / p.F;
-          piece.first = at - piece.index * p.F;
-          piece.count = min(min(64, p.F - piece.first), end - at);
-          at += piece.count;
-          break;
-        }
-        const int from = shared_column(at), to = shared_column(end);
-        piece.index = active;
-        piece.first = from;
-        piece.count = min(64, to - from);
-        at = piece.count > 0 && from + piece.count < to ? active * p.F + shared_weight() * (from + piece.count) : end;
-        if (piece.count > 0) break;
-      }
+  __device__ bool next() {
+    if (waiting > 0) {
+      piece.begin += piece.n;
+    } else if (!next_columns()) {
+      return false;
     }
-    const bool shared = piece.index == active;
-    piece.fp8 = p.fp8 && !shared;
-    piece.begin = shared ? 0 : l.begin[piece.index];
-    piece.n = shared ? p.T : l.begin[piece.index + 1] - piece.begin;
+    piece.n = min(waiting, kPassTokens);
+    waiting -= piece.n;
+    piece.ks_log = 0;
+    while (piece.ks_log + piece.rt_log < 4 && (2 << piece.ks_log) * piece.n <= p.b_rows) ++piece.ks_log;
+    piece.steps = (piece.blocks + (1 << piece.ks_log) - 1) >> piece.ks_log;
+    return true;
+  }
+  __device__ bool next_columns() {
+    if (at >= end) return false;
+    const int most = DOWN ? 256 : 128;
+    if (at < active * width()) {
+      piece.index = at / width();
+      piece.first = at - piece.index * width();
+      piece.count = min(min(most, width() - piece.first), end - at);
+      at += piece.count;
+      piece.fp8 = p.fp8;
+      piece.begin = l.begin[piece.index];
+      waiting = l.begin[piece.index + 1] - piece.begin;
+    } else {
+      piece.index = active;
+      piece.first = shared_column(at);
+      const int last = shared_column(end);
+      piece.count = min(most, last - piece.first);
+      if (piece.count <= 0) return false;
+      at = piece.first + piece.count < last ? active * width() + shared_cost() * (piece.first + piece.count) : end;
+      piece.fp8 = false;
+      piece.begin = 0;
+      waiting = p.T;
+    }
     const int tiles = DOWN ? (piece.count + 15) / 16 : (piece.count + 7) / 8;
     piece.rt_log = tiles <= 1 ? 0 : 32 - __clz(tiles - 1);
-    piece.ks_log = 0;
-    while (piece.ks_log + piece.rt_log < 3 && (2 << piece.ks_log) * piece.n <= p.b_rows) ++piece.ks_log;
     piece.blocks = (inner() * (piece.fp8 ? 1 : 2) + 127) / 128;
-    piece.steps = (piece.blocks + (1 << piece.ks_log) - 1) >> piece.ks_log;
+    return true;
   }
-  __device__ int inner() const { return DOWN ? (piece.index == active ? p.shared_inner : p.F) : p.D; }
-  __device__ void advance() {
-    if (++step == piece.steps) open();
-  }
+  __device__ int inner() const { return !DOWN ? p.D : piece.index == active ? p.shared_inner : p.F; }
 };
 
-// Fills stages: the next stage's weights, scales and tokens.
+// Where the K slices of a tile meet: a value of every lane for each of at most 16 tokens (a pass of more has one slice).
+__host__ __device__ inline int meet_bytes(int T) { return kMultiplyWarps * 32 * 4 * (T <= 8 ? 4 : 8); }
+
+struct Barriers {
+  uint64_t full[kMaxStages], empty[kMaxStages];
+  int abort;
+};
+
+// A stage's weights: [K block][row], UP: the piece's gate rows, then its up rows, in whole tiles; rows of 128 bytes.
+// Its tokens: [K block][token], and one scale each beside E4M3 weights; two of the weights' scales for each slab.  Fill
+// warp w has stages w, w + 4, ...: its first lane sends for the boxes, all its lanes bring the scales and the tokens'
+// columns.  There are at least as many stages as fill warps: a warp that fills stage s has filled s - 4, so
+// s - 4 - count has been read and a wait for s - count cannot take the phase before that one for it.
 template <bool DOWN>
-struct Loader : Stream<DOWN> {
-  const uint8_t* src[4];  // this thread's four chunks of 16 bytes
-  uint32_t has;           // which of them exist
-  const float* scale;     // and its scale, per K block
-  using Stream<DOWN>::p;
-  using Stream<DOWN>::l;
-  using Stream<DOWN>::piece;
+__device__ __forceinline__ void keep_full(const DecodeParams& p, const DecodeMaps& maps, const Lists& l, int active,
+                                          uint8_t* stages, uint8_t* token_stages, float* token_scales,
+                                          float* weight_scales, int count, Barriers& bars) {
+  const int lane = threadIdx.x & 31, turn = (threadIdx.x >> 5) - kMultiplyWarps;
+  Stream<DOWN> now(p, l, active);
+  int slot = 0, stage = 0;
+  uint32_t phase = 0;
+  bool dead = false;
+  while (!dead && now.next()) {
+    const Piece& piece = now.piece;
+    const bool shared = piece.index == active;
+    const CUtensorMap* tall = shared ? &maps.shared_tall : &maps.tall;
+    const CUtensorMap* flat = shared ? &maps.shared_flat : &maps.flat;
+    const int inner = now.inner(), ks_count = 1 << piece.ks_log;
+    const int columns = piece.fp8 ? 128 : 64;  // of a K block
+    const int up = shared ? p.shared_inner : p.F;
+    const int y = (shared ? 0 : l.expert[piece.index] * (DOWN ? p.D : 2 * p.F)) + piece.first;
+    const int block_bytes = kSlab << piece.rt_log;
+    const __nv_bfloat16* tokens = !DOWN ? p.x : (shared ? p.act_shared : p.act) + (long long)piece.begin * inner;
+    // a lane has the scale of half `lane & 1` of slab `lane >> 1`
+    const float* scale = nullptr;
+    const int scale_ks = lane >> (1 + piece.rt_log);
+    if (piece.fp8) {
+      const int rt = (lane >> 1) & ((1 << piece.rt_log) - 1), rows = DOWN ? p.D : p.F;
+      const int column = min(piece.first + rt * (DOWN ? 16 : 8) + (DOWN ? (lane & 1) * 8 : 0), rows - 1);
+      const int row = column + (DOWN ? 0 : (lane & 1) * p.F);
+      scale = (DOWN ? p.w2_scale : p.w13_scale) +
+              ((long long)l.expert[piece.index] * ((DOWN ? p.D : 2 * p.F) >> 7) + (row >> 7)) * piece.blocks + scale_ks;
+    }
+    for (int step = 0; step < piece.steps; ++step, ++stage) {
+      if ((stage & (kFillWarps - 1)) == turn) {
+        const int block0 = step << piece.ks_log, here = min(ks_count, piece.blocks - block0);  // K blocks of this stage
+        const int rows = here * piece.n;
+        if (stage >= count && !wait_stage(&bars.empty[slot], phase ^ 1, &bars.abort, p.status, 70)) {
+          dead = true;
+          break;
+        }
+        if (scale != nullptr && scale_ks < here) copy4(weight_scales + slot * kStageScales + lane, scale + block0);
+        uint64_t* full = &bars.full[slot];
+        if (lane == 0) {
+          uint8_t* to = stages + slot * kStageA;
+          mbar_arrive_expect_tx(full, here * piece.count * (DOWN ? 128 : 256));
+          for (int ks = 0; ks < here; ++ks, to += block_bytes) {
+            const int x = (block0 + ks) * columns;
+            if (DOWN) {
+              if (piece.count == 256) {
+                tma_load_2d(to, tall, full, x, y);
+              } else {
+                for (int row = 0; row < piece.count; row += 8) tma_load_2d(to + row * 128, flat, full, x, y + row);
+              }
+            } else if (piece.count == 128) {
+              tma_load_2d(to, tall, full, x, y);
+              tma_load_2d(to + 16384, tall, full, x, y + up);
+            } else {
+              for (int row = 0; row < piece.count; row += 8) {
+                tma_load_2d(to + row * 128, flat, full, x, y + row);
+                tma_load_2d(to + block_bytes / 2 + row * 128, flat, full, x, y + up + row);
+              }
+            }
+          }
+        }
+        __syncwarp();
+        uint8_t* b = token_stages + slot * p.b_rows * kTokenBytes;
+        float* scales = token_scales + slot * p.b_rows;
+        if (!piece.fp8) {
+          for (int i = lane; i < rows * 8; i += 32) {
+            const int at = i >> 3, ks = here == 1 ? 0 : at / piece.n, row = at - ks * piece.n;
+            const int token = DOWN ? row : shared ? piece.begin + row : l.tokens[piece.begin + row];
+            const int k = (block0 + ks) * 64 + (i & 7) * 8;  // behind the end of a row: zeros, as the boxes have
+            copy16(b + at * kTokenPitchBf16 + (i & 7) * 16, tokens + (long long)token * inner + (k < inner ? k : 0),
+                   k < inner);
+          }
+        } else {
+          for (int i = lane; i < rows * 16; i += 32) {
+            const int at = i >> 4, ks = here == 1 ? 0 : at / piece.n, row = at - ks * piece.n;
+            const long long from =
+                (long long)(DOWN ? piece.begin + row : l.tokens[piece.begin + row]) * piece.blocks + block0 + ks;
+            copy16(b + at * kTokenBytes + (((i & 15) ^ (row & 1)) << 4),
+                   (DOWN ? p.act16 : p.x16) + from * kTokenBytes + (i & 15) * 16, true);
+            if ((i & 15) == 0) copy4(scales + at, (DOWN ? p.act16_scale : p.x16_scale) + from);
+          }
+        }
+        copies_arrive(full);
+      }
+      if (++slot == count) {
+        slot = 0;
+        phase ^= 1;
+      }
+    }
+  }
+  if (dead) {  // nothing of this warp's may still be on its way when it leaves
+    volatile int go_on = 0;
+    for (int i = 1; i <= min(stage, count); ++i) {
+      slot = slot == 0 ? count - 1 : slot - 1;
+      if (slot == count - 1) phase ^= 1;
+      if (((stage - i) & (kFillWarps - 1)) == turn && lane == 0) mbar_wait(&bars.full[slot], phase, &go_on, p.status, 71);
+    }
+    __syncwarp();
+  }
+}
 
-  __device__ Loader(const DecodeParams& params, const Lists& lists, int n_active)
-      : Stream<DOWN>(params, lists, n_active) {
-    aim();
-  }
-  // the weight row behind row `r` of tile `rt`, or -1
-  __device__ int weight_row(int rt, int r) const {
-    if (DOWN) {
-      const int row = rt * 16 + r;
-      return row < piece.count ? piece.first + row : -1;
-    }
-    const int column = rt * 8 + (r & 7);
-    const int half = piece.index == this->active ? p.shared_inner : p.F;
-    return column < piece.count ? (r >> 3) * half + piece.first + column : -1;
-  }
-  __device__ void aim() {
-    if (this->done) return;
-    const bool shared = piece.index == this->active;
-    const int inner = this->inner();
-    const long long pitch = (long long)inner * (piece.fp8 ? 1 : 2);
-    const uint8_t* base = DOWN ? (shared ? p.shared_w2 : p.w2) : (shared ? p.shared_w13 : p.w13);
-    const float* scales = DOWN ? p.w2_scale : p.w13_scale;
-    if (!shared) {
-      const long long e = l.expert[piece.index], rows = DOWN ? p.D : 2LL * p.F;
-      base += e * rows * pitch;
-      if (piece.fp8) scales += e * (rows / 128) * piece.blocks;
-    }
-    const int tid = threadIdx.x, r = (tid >> 3) & 15;
-    has = 0;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int slab = (tid >> 7) + 2 * i, rt = slab & ((1 << piece.rt_log) - 1), ks = slab >> piece.rt_log;
-      const int row = ks < (1 << piece.ks_log) ? weight_row(rt, r) : -1;
-      src[i] = base + (row < 0 ? 0 : row) * pitch + ks * 128 + (tid & 7) * 16;
-      if (row >= 0) has |= 1u << i;
-    }
-    if (tid < 128) {
-      const int slab = tid >> 4, rt = slab & ((1 << piece.rt_log) - 1), ks = slab >> piece.rt_log;
-      const int row = piece.fp8 && ks < (1 << piece.ks_log) ? weight_row(rt, tid & 15) : -1;
-      scale = row < 0 ? nullptr : scales + (long long)(row >> 7) * piece.blocks + ks;
-    }
-  }
-  __device__ void fill(uint8_t* stage) {
-    if (!this->done) {
-      const int tid = threadIdx.x, inner = this->inner(), ks_count = 1 << piece.ks_log;
-      const int block0 = this->step << piece.ks_log;  // first K block of the stage
-      const int pitch = inner * (piece.fp8 ? 1 : 2);
-      const int r = (tid >> 3) & 15;
-      const int to = r * 128 + (((tid & 7) ^ ((r & 1) << 2)) << 4);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int slab = (tid >> 7) + 2 * i, block = block0 + (slab >> piece.rt_log);
-        const bool in = block * 128 + (tid & 7) * 16 < pitch;  // zeros behind the end of a row
-        if (((has >> i) & 1) && block < piece.blocks)
-          copy16(stage + slab * kSlab + to, in ? src[i] : (const uint8_t*)p.x, in);
-        src[i] += ks_count * 128;
-      }
-      if (tid < 128) {
-        if (scale != nullptr && block0 + (tid >> (4 + piece.rt_log)) < piece.blocks)
-          copy4(stage + kStageA + tid * 4, scale);
-        scale += scale != nullptr ? ks_count : 0;
-      }
-      // the tokens' columns of the same K blocks: [K block][token][256 or 128 bytes]
-      const bool shared = piece.index == this->active;
-      const int chunk_log = piece.fp8 ? 4 : 3, total = (ks_count * piece.n) << chunk_log;
-      uint8_t* b = stage + kStageA + kStageScales;
-      for (int i = tid; i < total; i += kDecodeThreads) {
-        const int chunk = i & ((1 << chunk_log) - 1), at_row = i >> chunk_log;
-        const int ks = ks_count == 1 ? 0 : at_row / piece.n, row = at_row - ks * piece.n;
-        const int block = block0 + ks;
-        if (block >= piece.blocks) continue;
-        const int k = (block << (chunk_log + 3)) + chunk * 8;
-        const __nv_bfloat16* from;
-        if (DOWN)
-          from = shared ? p.act_shared + (long long)row * inner : p.act + (long long)(piece.begin + row) * inner;
-        else
-          from = p.x + (long long)(shared ? row : l.tokens[piece.begin + row]) * inner;
-        const int swizzle = piece.fp8 ? (row & 1) : (row & 1) << 2;
-        copy16(b + (at_row << (chunk_log + 4)) + ((chunk ^ swizzle) << 4), from + (k < inner ? k : 0), k < inner);
-      }
-      const int before = this->step;
-      this->advance();
-      if (this->step != before + 1) aim();
-    }
-    copies_commit();
-  }
-};
+// One warp's slab of a stage: 16 weight rows x 128 bytes of K by up to 8 * MOST tokens.  Lane (g, t) reads the same
+// 16 (bf16: 8) consecutive columns of its weight rows and of its token, which is one order of the columns for both
+// operands.  Rows behind the last token are read as that token's; their sums go nowhere.
+// Weight rows j and j + 4 of a box go to neighbouring lanes: under the 128-byte swizzle they lie in different banks.
+__device__ __forceinline__ int box_row(int g) { return (g >> 1) + ((g & 1) << 2); }
 
-// One warp's slab of a stage: 16 weight rows x 128 bytes of K by NT tiles of 8 tokens.  Lane (g, t) reads the
-// same 16 (bf16: 8) consecutive columns of its weight rows and of its token, which is one order of the columns
-// for both operands.  Rows behind the last token are read as that token's; their sums go nowhere.
-template <bool FP8, int NT>
-__device__ __forceinline__ void multiply(const uint8_t* slab, const float* scales, const uint8_t* b, int n,
-                                         float (&acc)[8][4]) {
-  const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-  const uint8_t* rows = slab + g * 128;
-  const int swizzle = (g & 1) << 2;
-  float part[NT][4];
-  if constexpr (FP8) {
-#pragma unroll
-    for (int i = 0; i < NT; ++i) part[i][0] = part[i][1] = part[i][2] = part[i][3] = 0.f;
-  }
+// acc[4 i + h], acc[4 i + 2 + h] are the sums of token 8 i + 2 t + h for the lane's two weight rows.
+template <int MOST>
+__device__ __forceinline__ void multiply_e4m3(const uint8_t* low, int high, float2 s, const uint8_t* b,
+                                              const float* scales, int n, float (&acc)[MOST * 4]) {
+  const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3, row = box_row(g);
+  const uint8_t* rows = low + row * 128;  // the other eight rows are `high` bytes further
 #pragma unroll
   for (int segment = 0; segment < 2; ++segment) {
-    const int at = ((segment * 4 + t) ^ swizzle) << 4;
+    const int at = ((segment * 4 + t) ^ row) << 4;
     const uint4 lo = *reinterpret_cast<const uint4*>(rows + at);
-    const uint4 hi = *reinterpret_cast<const uint4*>(rows + 1024 + at);
-    if constexpr (FP8) {
-      uint32_t a[4][4];
+    const uint4 hi = *reinterpret_cast<const uint4*>(rows + high + at);
+    uint32_t a[4][4];
+    widen(lo.x, a[0][0], a[0][2]), widen(hi.x, a[0][1], a[0][3]);
+    widen(lo.y, a[1][0], a[1][2]), widen(hi.y, a[1][1], a[1][3]);
+    widen(lo.z, a[2][0], a[2][2]), widen(hi.z, a[2][1], a[2][3]);
+    widen(lo.w, a[3][0], a[3][2]), widen(hi.w, a[3][1], a[3][3]);
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        a[j][0] = widen2(word(lo, j));
-        a[j][1] = widen2(word(hi, j));
-        a[j][2] = widen2(word(lo, j) >> 16);
-        a[j][3] = widen2(word(hi, j) >> 16);
-      }
-#pragma unroll
-      for (int i = 0; i < NT; ++i) {
-        const int row = min(i * 8 + g, n - 1), chunk = segment * 8 + 2 * t;
-        const uint4 v0 = *reinterpret_cast<const uint4*>(b + row * 256 + ((chunk ^ (row & 1)) << 4));
-        const uint4 v1 = *reinterpret_cast<const uint4*>(b + row * 256 + (((chunk + 1) ^ (row & 1)) << 4));
-        mma_bf16(part[i], a[0][0], a[0][1], a[0][2], a[0][3], v0.x, v0.y);
-        mma_bf16(part[i], a[1][0], a[1][1], a[1][2], a[1][3], v0.z, v0.w);
-        mma_bf16(part[i], a[2][0], a[2][1], a[2][2], a[2][3], v1.x, v1.y);
-        mma_bf16(part[i], a[3][0], a[3][1], a[3][2], a[3][3], v1.z, v1.w);
-      }
-    } else {
-#pragma unroll
-      for (int i = 0; i < NT; ++i) {
-        const int row = min(i * 8 + g, n - 1);
-        const uint4 v = *reinterpret_cast<const uint4*>(b + row * 128 + (((segment * 4 + t) ^ ((row & 1) << 2)) << 4));
-        mma_bf16(acc[i], lo.x, hi.x, lo.y, hi.y, v.x, v.y);
-        mma_bf16(acc[i], lo.z, hi.z, lo.w, hi.w, v.z, v.w);
+    for (int i = 0; i < MOST; ++i) {
+      if (i * 8 < n) {
+        const int token = min(i * 8 + g, n - 1), chunk = (segment * 8 + 2 * t) ^ (token & 1);
+        const uint4 v0 = *reinterpret_cast<const uint4*>(b + token * kTokenBytes + (chunk << 4));
+        const uint4 v1 = *reinterpret_cast<const uint4*>(b + token * kTokenBytes + ((chunk ^ 1) << 4));
+        float c[4] = {0.f, 0.f, 0.f, 0.f};
+        mma_f16(c, a[0][0], a[0][1], a[0][2], a[0][3], v0.x, v0.y);
+        mma_f16(c, a[1][0], a[1][1], a[1][2], a[1][3], v0.z, v0.w);
+        mma_f16(c, a[2][0], a[2][1], a[2][2], a[2][3], v1.x, v1.y);
+        mma_f16(c, a[3][0], a[3][1], a[3][2], a[3][3], v1.z, v1.w);
+        const float t0 = scales[min(i * 8 + 2 * t, n - 1)], t1 = scales[min(i * 8 + 2 * t + 1, n - 1)];
+        acc[4 * i] = fmaf(c[0], s.x * t0, acc[4 * i]);
+        acc[4 * i + 1] = fmaf(c[1], s.x * t1, acc[4 * i + 1]);
+        acc[4 * i + 2] = fmaf(c[2], s.y * t0, acc[4 * i + 2]);
+        acc[4 * i + 3] = fmaf(c[3], s.y * t1, acc[4 * i + 3]);
       }
     }
   }
-  if constexpr (FP8) {
-    const float s0 = scales[g], s1 = scales[g + 8];
+}
+
+// The same on bf16 weights.
+template <int MOST>
+__device__ __forceinline__ void multiply_bf16(const uint8_t* low, int high, const uint8_t* b, int n,
+                                              float (&acc)[MOST * 4]) {
+  const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3, row = box_row(g);
+  uint4 lo[2], hi[2];
 #pragma unroll
-    for (int i = 0; i < NT; ++i) {
-      acc[i][0] = fmaf(part[i][0], s0, acc[i][0]);
-      acc[i][1] = fmaf(part[i][1], s0, acc[i][1]);
-      acc[i][2] = fmaf(part[i][2], s1, acc[i][2]);
-      acc[i][3] = fmaf(part[i][3], s1, acc[i][3]);
+  for (int segment = 0; segment < 2; ++segment) {
+    const uint8_t* at = low + row * 128 + (((segment * 4 + t) ^ row) << 4);
+    lo[segment] = *reinterpret_cast<const uint4*>(at);
+    hi[segment] = *reinterpret_cast<const uint4*>(at + high);
+  }
+#pragma unroll
+  for (int i = 0; i < MOST; ++i) {
+    if (i * 8 < n) {
+      const uint8_t* token = b + min(i * 8 + g, n - 1) * kTokenPitchBf16 + t * 16;
+      const uint4 v0 = *reinterpret_cast<const uint4*>(token), v1 = *reinterpret_cast<const uint4*>(token + 64);
+      float(&c)[4] = *reinterpret_cast<float(*)[4]>(&acc[4 * i]);
+      mma_bf16(c, lo[0].x, hi[0].x, lo[0].y, hi[0].y, v0.x, v0.y);
+      mma_bf16(c, lo[0].z, hi[0].z, lo[0].w, hi[0].w, v0.z, v0.w);
+      mma_bf16(c, lo[1].x, hi[1].x, lo[1].y, hi[1].y, v1.x, v1.y);
+      mma_bf16(c, lo[1].z, hi[1].z, lo[1].w, hi[1].w, v1.z, v1.w);
     }
   }
 }
@@ -517,161 +623,179 @@ __device__ __forceinline__ float gated(float gate, float up, int limited, float 
   return gate * __frcp_rn(1.0f + expf(-gate)) * up;
 }
 
-template <bool DOWN, int STAGES>
-__global__ void __launch_bounds__(kDecodeThreads, 2)
-stream_kernel(const DecodeParams p) {
-  extern __shared__ __align__(128) uint8_t shared_memory[];
+// MOST: groups of 8 tokens that a pass can have.
+template <bool DOWN, int MOST>
+__global__ void __launch_bounds__(kStreamThreads, 1)
+stream_kernel(const DecodeParams p, const __grid_constant__ DecodeMaps maps, int stages) {
+  extern __shared__ __align__(1024) uint8_t shared_memory[];
+  __shared__ Barriers bars;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
-  const int stage_bytes = kStageA + kStageScales + p.b_rows * 256;
-  uint8_t* behind = shared_memory + STAGES * stage_bytes;
-  float* sums = reinterpret_cast<float*>(behind);  // DOWN: [slab][token][16 output columns]
-  Lists l;
-  l.place(behind + (DOWN ? 8 * 16 * 4 * p.T : 0), p.T, p.E, p.K);
-  const int active = build_lists(l, p.ids, p.route_weights, p.T, p.E, p.K);
-  if (DOWN) {
-    for (int i = tid; i < 8 * 16 * p.T; i += kDecodeThreads) sums[i] = 0.f;
-    __syncthreads();
+  uint8_t* token_stages = shared_memory + stages * kStageA;
+  float* token_scales = reinterpret_cast<float*>(token_stages + stages * p.b_rows * kTokenBytes);
+  float* weight_scales = token_scales + stages * p.b_rows;
+  float* meet = weight_scales + stages * kStageScales;  // [slab][value][lane]
+  __shared__ Lists l;  // (in shared memory: its pointers took ten registers)
+  if (tid == 0) {
+    l.place(reinterpret_cast<uint8_t*>(meet) + meet_bytes(p.T), p.T, p.E, p.K);
+    for (int i = 0; i < stages; ++i) {
+      mbar_init(&bars.full[i], 1 + 32);  // boxes and copies
+      mbar_init(&bars.empty[i], kMultiplyWarps);
+    }
+    bars.abort = 0;
+    fence_mbar_init();
+    tma_prefetch_desc(&maps.tall);
+    tma_prefetch_desc(&maps.flat);
+  }
+  __syncthreads();
+  const int active = build_lists(l, p.ids, p.T, p.E, p.K, !DOWN && blockIdx.x == 0 ? p.row_of : nullptr);
+  if (warp >= kMultiplyWarps) {
+    keep_full<DOWN>(p, maps, l, active, shared_memory, token_stages, token_scales, weight_scales, stages, bars);
+    return;
   }
 
-  Loader<DOWN> loader(p, l, active);
+  const auto meet_all = [] { named_sync(1, 32 * kMultiplyWarps); };  // the multiplying warps
   Stream<DOWN> now(p, l, active);
-  for (int i = 0; i < STAGES - 1; ++i) loader.fill(shared_memory + i * stage_bytes);
-  float acc[8][4];
-#pragma unroll
-  for (int i = 0; i < 8; ++i) acc[i][0] = acc[i][1] = acc[i][2] = acc[i][3] = 0.f;
   int slot = 0;
-  while (!now.done) {
-    copies_wait<STAGES - 2>();
-    __syncthreads();  // this stage is there for everybody, and the one before it is free
-    loader.fill(shared_memory + (slot == 0 ? STAGES - 1 : slot - 1) * stage_bytes);
-    const Piece piece = now.piece;
-    uint8_t* stage = shared_memory + slot * stage_bytes;
-    const int rt = warp & ((1 << piece.rt_log) - 1), ks = warp >> piece.rt_log;
-    const bool mine = ks < (1 << piece.ks_log) && rt * (DOWN ? 16 : 8) < piece.count;
-    const int block = (now.step << piece.ks_log) + ks, tiles = (piece.n + 7) >> 3;
-    if (mine && block < piece.blocks) {
-      const uint8_t* slab = stage + warp * kSlab;
-      const float* scales = reinterpret_cast<const float*>(stage + kStageA) + warp * 16;
-      const uint8_t* b = stage + kStageA + kStageScales + ((ks * piece.n) << (piece.fp8 ? 8 : 7));
-      if (piece.fp8) {
-        if (tiles == 1) multiply<true, 1>(slab, scales, b, piece.n, acc);
-        else if (tiles == 2) multiply<true, 2>(slab, scales, b, piece.n, acc);
-        else if (tiles <= 4) multiply<true, 4>(slab, scales, b, piece.n, acc);
-        else multiply<true, 8>(slab, scales, b, piece.n, acc);
-      } else {
-        if (tiles == 1) multiply<false, 1>(slab, scales, b, piece.n, acc);
-        else if (tiles == 2) multiply<false, 2>(slab, scales, b, piece.n, acc);
-        else if (tiles <= 4) multiply<false, 4>(slab, scales, b, piece.n, acc);
-        else multiply<false, 8>(slab, scales, b, piece.n, acc);
+  uint32_t phase = 0;
+  bool dead = false;  // a wait ran out: go on to the end without waiting, the status says so
+  while (now.next()) {
+    const Piece& piece = now.piece;
+    const bool is_shared = piece.index == active;
+    constexpr int kTile = DOWN ? 16 : 8;  // output columns
+    const int rt = warp & ((1 << piece.rt_log) - 1), ks = warp >> piece.rt_log, ks_count = 1 << piece.ks_log;
+    const bool mine = ks < ks_count && rt * kTile < piece.count;
+    // this lane's two weight rows are `column` and, 8 further (DOWN) or the up row of the same column (UP)
+    const int column = rt * kTile + box_row(g);
+    const int low = (ks << piece.rt_log) * kSlab + rt * (DOWN ? 2048 : 1024), high = DOWN ? 1024 : 1024 << piece.rt_log;
+    const int first_token = ks * piece.n;
+    float acc[MOST * 4];
+#pragma unroll
+    for (int i = 0; i < MOST * 4; ++i) acc[i] = 0.f;
+    int block = ks;
+    for (int step = 0; step < piece.steps; ++step, block += ks_count) {
+      if (!dead) dead = !wait_stage(&bars.full[slot], phase, &bars.abort, p.status, 72);
+      if (mine && block < piece.blocks) {
+        const uint8_t* a = shared_memory + slot * kStageA + low;
+        const uint8_t* b = token_stages + slot * p.b_rows * kTokenBytes;
+        if (piece.fp8)
+          multiply_e4m3<MOST>(a, high, reinterpret_cast<const float2*>(weight_scales + slot * kStageScales)[warp],
+                              b + first_token * kTokenBytes, token_scales + slot * p.b_rows + first_token, piece.n, acc);
+        else
+          multiply_bf16<MOST>(a, high, b + first_token * kTokenPitchBf16, piece.n, acc);
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&bars.empty[slot]);
+      if (++slot == stages) {
+        slot = 0;
+        phase ^= 1;
       }
     }
-    const int step = now.step;
-    now.advance();
-    if (step + 1 == piece.steps) {  // the piece's sums are complete
-      const bool is_shared = piece.index == active;
-      if (DOWN) {
-        if (mine) {
-          float* to = sums + warp * 16 * p.T;
+    // The piece's sums are complete.
+    if (ks_count > 1) {  // the warps of a tile add up
+      const int used = 4 * ((piece.n + 7) >> 3);
+      meet_all();
+      if (mine && ks > 0) {
 #pragma unroll
-          for (int i = 0; i < 8; ++i) {
+        for (int i = 0; i < MOST * 4; ++i)
+          if (i < used) meet[(warp * used + i) * 32 + lane] = acc[i];
+      }
+      meet_all();
+      if (mine && ks == 0) {
+        for (int s = 1; s < ks_count; ++s)
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
-              const int j = i * 8 + 2 * t + h;
-              if (j < piece.n) {
-                const int token = is_shared ? j : l.tokens[piece.begin + j];
-                const float w = is_shared ? 1.0f : l.weights[piece.begin + j];
-                float* at = to + token * 16 + g;
-                at[0] = fmaf(w, acc[i][h], at[0]);
-                at[8] = fmaf(w, acc[i][2 + h], at[8]);
-              }
-            }
+          for (int i = 0; i < MOST * 4; ++i)
+            if (i < used) acc[i] += meet[(((s << piece.rt_log) + rt) * used + i) * 32 + lane];
+      }
+    }
+    if (mine && ks == 0 && column < piece.count) {
+      const int width = DOWN ? p.D : is_shared ? p.shared_inner : p.F;
+#pragma unroll
+      for (int q = 0; q < MOST * 2; ++q) {
+        const int j = (q >> 1) * 8 + 2 * t + (q & 1);
+        const float first = acc[(q >> 1) * 4 + (q & 1)], second = acc[(q >> 1) * 4 + 2 + (q & 1)];
+        if (j < piece.n) {
+          const long long at = (long long)(piece.begin + j) * width + piece.first + column;
+          if (DOWN) {
+            float* to = p.y + (is_shared ? (long long)p.T * p.K * p.D : 0) + at;
+            to[0] = first;
+            if (column + 8 < piece.count) to[8] = second;
+          } else {
+            (is_shared ? p.act_shared : p.act)[at] = __float2bfloat16_rn(gated(first, second, p.limited, p.limit));
           }
-        }
-        __syncwarp();  // the next expert may give this warp's sums to other lanes
-        if (now.done || now.piece.first != piece.first) {  // the last expert of these columns
-          __syncthreads();
-          for (int i = tid; i < p.T << (piece.rt_log + 4); i += kDecodeThreads) {
-            const int column = i & ((16 << piece.rt_log) - 1), token = i >> (piece.rt_log + 4);
-            if (column < piece.count) {
-              const long long at = (long long)token * p.D + piece.first + column;
-              float v = __bfloat162float(p.residual[at]);
-              for (int s = column >> 4; s < 8; s += 1 << piece.rt_log) v += sums[(s * p.T + token) * 16 + (column & 15)];
-              p.out[at] = __float2bfloat16_rn(v);
-            }
-          }
-          __syncthreads();
-          for (int i = tid; i < 8 * 16 * p.T; i += kDecodeThreads) sums[i] = 0.f;
-          __syncthreads();
-        }
-      } else {
-        if (piece.ks_log > 0) {  // the warps of a tile meet in the stage that has just been read
-          float* meet = reinterpret_cast<float*>(stage);
-          __syncthreads();
-          if (mine && ks > 0) {
-#pragma unroll
-            for (int i = 0; i < 8; ++i)
-              if (i < tiles)
-#pragma unroll
-                for (int h = 0; h < 4; ++h) meet[((warp * tiles + i) * 4 + h) * 32 + lane] = acc[i][h];
-          }
-          __syncthreads();
-          if (mine && ks == 0) {
-            for (int s = 1; s < 1 << piece.ks_log; ++s)
-#pragma unroll
-              for (int i = 0; i < 8; ++i)
-                if (i < tiles)
-#pragma unroll
-                  for (int h = 0; h < 4; ++h)
-                    acc[i][h] += meet[((((s << piece.rt_log) + rt) * tiles + i) * 4 + h) * 32 + lane];
-          }
-        }
-        const int column = rt * 8 + g;
-        if (mine && ks == 0 && column < piece.count) {
-          const int width = is_shared ? p.shared_inner : p.F;
-          __nv_bfloat16* to = (is_shared ? p.act_shared : p.act + (long long)piece.begin * p.F) + piece.first + column;
-#pragma unroll
-          for (int i = 0; i < 8; ++i)
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-              const int j = i * 8 + 2 * t + h;
-              if (j < piece.n)
-                to[(long long)j * width] = __float2bfloat16_rn(gated(acc[i][h], acc[i][2 + h], p.limited, p.limit));
-            }
         }
       }
-#pragma unroll
-      for (int i = 0; i < 8; ++i) acc[i][0] = acc[i][1] = acc[i][2] = acc[i][3] = 0.f;
     }
-    slot = slot + 1 == STAGES ? 0 : slot + 1;
   }
-  copies_wait<0>();
+}
+
+// act [rows, F] for the E4M3 down product: f16 with a power of two per 128 columns, a warp to a block.
+__global__ void __launch_bounds__(kDecodeThreads)
+scale_act_kernel(const __nv_bfloat16* __restrict__ act, int blocks, uint8_t* __restrict__ act16,
+                 float* __restrict__ act16_scale) {
+  const int i = blockIdx.x * kDecodeWarps + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+  if (i >= blocks) return;
+  uint2 scaled;
+  const float scale = scale_block(reinterpret_cast<const uint2*>(act)[(long long)i * 32 + lane], scaled);
+  reinterpret_cast<uint2*>(act16)[(long long)i * 32 + lane] = scaled;
+  if (lane == 0) act16_scale[i] = scale;
+}
+
+// out[t] = residual[t] + sum_k w[t,k] y[row_of[t,k]] (+ the shared expert's row of t): fp32, k ascending, one rounding.
+// A thread has four columns of a token.
+__global__ void __launch_bounds__(kDecodeThreads)
+join_kernel(const DecodeParams p) {
+  const int t = blockIdx.y, c = (blockIdx.x * kDecodeThreads + threadIdx.x) * 4;
+  if (c >= p.D) return;
+  const long long at = (long long)t * p.D + c;
+  float v[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) v[i] = __bfloat162float(p.residual[at + i]);
+  for (int k = 0; k < p.K; ++k) {
+    const float w = p.route_weights[t * p.K + k];
+    const float4 y = *reinterpret_cast<const float4*>(p.y + (long long)p.row_of[t * p.K + k] * p.D + c);
+    v[0] = fmaf(w, y.x, v[0]), v[1] = fmaf(w, y.y, v[1]), v[2] = fmaf(w, y.z, v[2]), v[3] = fmaf(w, y.w, v[3]);
+  }
+  if (p.shared_inner > 0) {
+    const float4 y = *reinterpret_cast<const float4*>(p.y + (long long)(p.T * p.K + t) * p.D + c);
+    v[0] += y.x, v[1] += y.y, v[2] += y.z, v[3] += y.w;
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) p.out[at + i] = __float2bfloat16_rn(v[i]);
 }
 
 struct DecodeWorkspace {
-  long long logits, act, act_shared, bytes;
-  DecodeWorkspace(long long T, long long E, long long K, long long F, long long shared_inner) {
+  long long logits, x16, x16_scale, act, act_shared, act16, act16_scale, y, row_of, bytes;
+  DecodeWorkspace(long long T, long long D, long long E, long long K, long long F, long long shared_inner) {
     const auto up = [](long long n) { return (n + 255) / 256 * 256; };
     logits = 0;
-    act = up(4 * T * E);
+    x16 = up(4 * T * E);
+    x16_scale = x16 + up(T * (D / 128) * kTokenBytes);
+    act = x16_scale + up(4 * T * (D / 128));
     act_shared = act + up(2 * T * K * F);
-    bytes = act_shared + up(2 * T * shared_inner);
+    act16 = act_shared + up(2 * T * shared_inner);
+    act16_scale = act16 + up(T * K * (F / 128) * kTokenBytes);
+    y = act16_scale + up(4 * T * K * (F / 128));
+    row_of = y + up(4 * (T * K + (shared_inner > 0 ? T : 0)) * D);
+    bytes = row_of + up(4 * T * K);
   }
 };
 
 static int decode_sizes(long long tokens, int width, int inner, int experts, int top_k, int shared_inner) {
   if (tokens < 0 || width <= 0 || inner <= 0 || experts <= 0 || top_k <= 0 || top_k > experts || shared_inner < 0)
     return B200MOE_ERR_ARG;
-  if (tokens > kMaxTokens || experts > 1024 || top_k > 32 || width > (1 << 20) || inner > (1 << 20) ||
-      shared_inner > (1 << 20))
+  if (tokens > kMaxTokens || experts > 1024 || top_k > 32 || width > (1 << 19) || inner > (1 << 19) ||
+      shared_inner > (1 << 19))
     return B200MOE_ERR_LIMIT;
   if (width % 8 || inner % 8 || shared_inner % 8) return B200MOE_ERR_ALIGN;
   return B200MOE_OK;
 }
 
 template <typename W>
-static int launch_router(const b200moe_decode_args* a, float* logits, cudaStream_t s) {
+static int launch_router(const b200moe_decode_args* a, float* logits, uint8_t* x16, float* x16_scale,
+                         cudaStream_t s) {
   cudaLaunchConfig_t config = {};
-  config.gridDim = dim3((unsigned)((a->experts + 15) / 16 * kRouterCluster));
+  const int scaling = x16 != nullptr ? ((int)a->tokens + 15) / 16 : 0;  // clusters, a warp for each 128 columns of 16 tokens
+  config.gridDim = dim3((unsigned)(((a->experts + 15) / 16 + scaling) * kRouterCluster));
   config.blockDim = dim3(kDecodeThreads);
   config.stream = s;
   cudaLaunchAttribute attribute;
@@ -683,21 +807,48 @@ static int launch_router(const b200moe_decode_args* a, float* logits, cudaStream
   const auto kernel = a->tokens <= 8 ? router_logits_kernel<W, 1> : a->tokens <= 32 ? router_logits_kernel<W, 4>
                                                                                    : router_logits_kernel<W, 8>;
   return cudaLaunchKernelEx(&config, kernel, (const __nv_bfloat16*)a->x, (const W*)a->router, (int)a->tokens, a->experts,
-                            a->width, logits) == cudaSuccess
+                            a->width, logits, x16, x16_scale) == cudaSuccess
              ? launch_status()
              : B200MOE_ERR_LAUNCH;
 }
 
-template <bool DOWN, int STAGES>
-static int launch_stream(const DecodeParams& p, cudaStream_t s) {
-  const int bytes = STAGES * (kStageA + kStageScales + p.b_rows * 256) + (DOWN ? 8 * 16 * 4 * p.T : 0) +
-                    Lists::bytes(p.T, p.E, p.K);
-  const auto kernel = stream_kernel<DOWN, STAGES>;
+// [rows, k] weights in boxes of `height` rows x 128 bytes
+static int encode_weights(CUtensorMap* map, const void* base, bool fp8, long long rows, long long k, int height) {
+  const uint64_t dims[2] = {(uint64_t)k, (uint64_t)rows}, strides[1] = {(uint64_t)(k * (fp8 ? 1 : 2))};
+  const uint32_t box[2] = {fp8 ? 128u : 64u, (uint32_t)height};
+  return encode_tensor_map(map, fp8 ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, base, dims,
+                           strides, box, CU_TENSOR_MAP_SWIZZLE_128B);
+}
+
+template <bool DOWN, int MOST>
+static int launch_stream(const DecodeParams& p, const DecodeMaps& maps, cudaStream_t s) {
+  const int stage = kStageA + p.b_rows * (kTokenBytes + 4) + kStageScales * 4;
+  const int rest = meet_bytes(p.T) + Lists::bytes(p.T, p.E, p.K);
+  int stages = (225 * 1024 - rest) / stage;
+  if (stages > kMaxStages) stages = kMaxStages;
+  if (stages < kFillWarps) return B200MOE_ERR_LIMIT;
+  const int bytes = stages * stage + rest;
+  const auto kernel = stream_kernel<DOWN, MOST>;
   if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) != cudaSuccess) {
     cudaGetLastError();
     return B200MOE_ERR_LAUNCH;
   }
-  kernel<<<sm_count(), kDecodeThreads, bytes, s>>>(p);
+  kernel<<<sm_count(), kStreamThreads, bytes, s>>>(p, maps, stages);
+  return launch_status();
+}
+
+template <int MOST>
+static int launch_streams(const DecodeParams& p, const DecodeMaps& up, const DecodeMaps& down, cudaStream_t s) {
+  int code = launch_stream<false, MOST>(p, up, s);
+  if (code != B200MOE_OK) return code;
+  if (p.fp8) {
+    const int blocks = p.T * p.K * (p.F / 128);
+    scale_act_kernel<<<(blocks + kDecodeWarps - 1) / kDecodeWarps, kDecodeThreads, 0, s>>>(p.act, blocks, p.act16,
+                                                                                          p.act16_scale);
+  }
+  code = launch_stream<true, MOST>(p, down, s);
+  if (code != B200MOE_OK) return code;
+  join_kernel<<<dim3((p.D / 4 + kDecodeThreads - 1) / kDecodeThreads, p.T), kDecodeThreads, 0, s>>>(p);
   return launch_status();
 }
 
@@ -708,7 +859,7 @@ using namespace b200;
 extern "C" long long b200moe_decode_workspace_bytes(long long tokens, int width, int inner, int experts, int top_k,
                                                     int shared_inner) {
   if (decode_sizes(tokens, width, inner, experts, top_k, shared_inner) != B200MOE_OK) return -1;
-  return DecodeWorkspace(tokens, experts, top_k, inner, shared_inner).bytes;
+  return DecodeWorkspace(tokens, width, experts, top_k, inner, shared_inner).bytes;
 }
 
 extern "C" int b200moe_decode(const b200moe_decode_args* a, void* stream) {
@@ -722,7 +873,7 @@ extern "C" int b200moe_decode(const b200moe_decode_args* a, void* stream) {
   }
   const bool fp8 = a->w13_scale != nullptr;
   if (!a->x || !a->residual || !a->router || !a->w13 || !a->w2 || !a->route_weights || !a->ids || !a->output ||
-      !a->workspace || fp8 != (a->w2_scale != nullptr) ||
+      !a->workspace || !a->status || fp8 != (a->w2_scale != nullptr) ||
       (a->shared_inner > 0 && (!a->shared_w13 || !a->shared_w2)))
     return B200MOE_ERR_ARG;
   if (fp8 && (a->width % 128 || a->inner % 128)) return B200MOE_ERR_ALIGN;
@@ -732,11 +883,31 @@ extern "C" int b200moe_decode(const b200moe_decode_args* a, void* stream) {
     return B200MOE_ERR_ALIGN;
   if (a->tokens == 0) return B200MOE_OK;
 
-  const DecodeWorkspace w(a->tokens, a->experts, a->top_k, a->inner, a->shared_inner);
+  DecodeMaps up, down;
+  const long long E = a->experts, D = a->width, F = a->inner, Fs = a->shared_inner;
+  int code = B200MOE_OK;
+  const auto encode = [&](CUtensorMap& map, const void* weights, bool e4m3, long long rows, long long k, int height) {
+    if (code == B200MOE_OK) code = encode_weights(&map, weights, e4m3, rows, k, height);
+  };
+  encode(up.tall, a->w13, fp8, 2 * E * F, D, 128);
+  encode(up.flat, a->w13, fp8, 2 * E * F, D, 8);
+  encode(down.tall, a->w2, fp8, E * D, F, 256);
+  encode(down.flat, a->w2, fp8, E * D, F, 8);
+  if (Fs > 0) {
+    encode(up.shared_tall, a->shared_w13, false, 2 * Fs, D, 128);
+    encode(up.shared_flat, a->shared_w13, false, 2 * Fs, D, 8);
+    encode(down.shared_tall, a->shared_w2, false, D, Fs, 256);
+    encode(down.shared_flat, a->shared_w2, false, D, Fs, 8);
+  }
+  if (code != B200MOE_OK) return code;
+  const DecodeWorkspace w(a->tokens, a->width, a->experts, a->top_k, a->inner, a->shared_inner);
   char* base = reinterpret_cast<char*>(a->workspace);
   float* logits = reinterpret_cast<float*>(base + w.logits);
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
-  int code = a->router_is_fp32 ? launch_router<float>(a, logits, s) : launch_router<__nv_bfloat16>(a, logits, s);
+  uint8_t* x16 = fp8 ? reinterpret_cast<uint8_t*>(base + w.x16) : nullptr;
+  float* x16_scale = reinterpret_cast<float*>(base + w.x16_scale);
+  code = a->router_is_fp32 ? launch_router<float>(a, logits, x16, x16_scale, s)
+                           : launch_router<__nv_bfloat16>(a, logits, x16, x16_scale, s);
   if (code != B200MOE_OK) return code;
   code = b200moe_route_topk(logits, a->experts, (int)a->tokens, a->experts, a->top_k, a->mode, a->bias, a->n_group,
                             a->topk_group, a->routed_scaling, a->route_weights, a->ids, stream);
@@ -752,17 +923,19 @@ extern "C" int b200moe_decode(const b200moe_decode_args* a, void* stream) {
   p.w2_scale = a->w2_scale;
   p.shared_w13 = reinterpret_cast<const uint8_t*>(a->shared_w13);
   p.shared_w2 = reinterpret_cast<const uint8_t*>(a->shared_w2);
+  p.x16 = x16;
+  p.x16_scale = x16_scale;
   p.act = reinterpret_cast<__nv_bfloat16*>(base + w.act);
+  p.act16 = reinterpret_cast<uint8_t*>(base + w.act16);
+  p.act16_scale = reinterpret_cast<float*>(base + w.act16_scale);
+  p.y = reinterpret_cast<float*>(base + w.y);
+  p.row_of = reinterpret_cast<int*>(base + w.row_of);
   p.act_shared = reinterpret_cast<__nv_bfloat16*>(base + w.act_shared);
   p.out = reinterpret_cast<__nv_bfloat16*>(a->output);
   p.T = (int)a->tokens, p.D = a->width, p.F = a->inner, p.E = a->experts, p.K = a->top_k;
   p.shared_inner = a->shared_inner;
   p.fp8 = fp8, p.limited = a->limited, p.limit = a->limit;
-  p.b_rows = p.T < 8 ? 8 * p.T : 64;
-  if (p.T <= 4) {
-    code = launch_stream<false, 4>(p, s);
-    return code != B200MOE_OK ? code : launch_stream<true, 4>(p, s);
-  }
-  code = launch_stream<false, 5>(p, s);
-  return code != B200MOE_OK ? code : launch_stream<true, 5>(p, s);
+  p.b_rows = p.T <= 2 ? 16 * p.T : kPassTokens;
+  p.status = a->status;
+  return p.T <= 8 ? launch_streams<1>(p, up, down, s) : launch_streams<kPassTokens / 8>(p, up, down, s);
 }

@@ -1229,7 +1229,7 @@ def moe_decode(x, residual, router, w13, w2, *, top_k, mode, bias=None, n_group=
         0 if limit is None else 1, 1 if router.dtype == torch.float32 else 0, shared_inner, float(routed_scaling),
         0.0 if limit is None else float(limit), x.data_ptr(), residual.data_ptr(), router.data_ptr(), _ptr(bias),
         w13.data_ptr(), _ptr(s13), w2.data_ptr(), _ptr(s2), _ptr(shared13), _ptr(shared2), weights.data_ptr(),
-        ids.data_ptr(), output.data_ptr(), workspace.data_ptr())
+        ids.data_ptr(), output.data_ptr(), workspace.data_ptr(), status_block(device).data_ptr())
     check(lib.b200moe_decode(ctypes.byref(args), _stream()), "moe_decode")
     _count(4)
     return output, weights, ids

@@ -53,7 +53,8 @@ def test_the_entry_point_refuses_bad_arguments_before_any_launch():
         assert call(**{name: 4096 + 8}) == -2, name
     assert call(workspace=4096 + 128) == -2 and call(tokens=0) == 0
     assert lib.b200moe_decode_workspace_bytes(65, 256, 128, 8, 2, 0) == -1
-    assert lib.b200moe_decode_workspace_bytes(4, 256, 128, 8, 2, 128) == 256 + 2048 + 1024
+    with_shared = [lib.b200moe_decode_workspace_bytes(4, 256, 128, 8, 2, shared) for shared in (0, 128)]
+    assert with_shared[1] - with_shared[0] == 2 * 4 * 128 + 4 * 4 * 256  # its activation and its rows of y
 
 
 def test_the_wrapper_refuses_what_it_does_not_take():
