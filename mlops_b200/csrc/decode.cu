@@ -16,9 +16,9 @@
 //
 // The weights are the A operand of mma.sync.m16n8k16 (16 weight rows), the tokens the B operand (8 to a tile).
 // Against bf16 weights the tokens are bf16.  E4M3 weights are widened to f16, one instruction for two values, and a
-// token's block of 128 columns is f16 with a power of two per block that puts its largest value in [2^14, 2^15): every
-// bf16 value down to 2^-29 of the largest exactly, what is smaller within 2^-40 of it.  The 128 x 128 block scales and
-// the tokens' powers of two are applied in fp32 to the sums of one block.  (Widening to bf16 takes four
+// token is f16 with a power of two of its own that puts its largest value in [2^14, 2^15): every bf16 value down to 2^-29
+// of the largest exactly, what is smaller within 2^-40 of it.  The 128 x 128 block scales are applied in fp32 to the
+// sums of one block, the tokens' powers of two to the finished sums.  (Widening to bf16 takes four
 // instructions for two values, 200 of the 356 issue slots an SM has per 2 KB of weights at full HBM rate;
 // m16n8k32 on E4M3 operands widens them inside, again for every tile: 22 cycles against 8 of m16n8k16.)
 //
@@ -91,12 +91,17 @@ __device__ __forceinline__ bool wait_stage(uint64_t* bar, uint32_t parity, volat
   return __shfl_sync(0xffffffffu, ok, 0) != 0;
 }
 
-__device__ __forceinline__ void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
-                                        uint32_t b1) {
+__device__ __forceinline__ void mma_f16(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
   asm volatile(
       "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
       : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void mma_f16_from_zero(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+      : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.f));
 }
 __device__ __forceinline__ void mma_bf16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
                                          uint32_t b1) {
@@ -114,19 +119,36 @@ __device__ __forceinline__ void widen(uint32_t w, uint32_t& first, uint32_t& sec
       : "r"(w));
 }
 
-// A warp scales 128 bf16 values, four to a lane, to f16 by the block's power of two (see the top), which it returns.
-__device__ __forceinline__ float scale_block(const uint2& raw, uint2& out) {
-  uint32_t m = __vmaxu2(raw.x & 0x7fff7fffu, raw.y & 0x7fff7fffu);
+// A block scales a row of bf16 to f16 by the row's power of two (see the top), which it returns to thread 0.  Infinities
+// and NaN stay what they are.  `width` is a multiple of 4; `largest` is scratch, one word per warp.
+__device__ __forceinline__ float scale_row(const __nv_bfloat16* __restrict__ from, int width, __half* __restrict__ to,
+                                           uint32_t* largest) {
+  const uint2* in = reinterpret_cast<const uint2*>(from);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  uint32_t m = 0;
+#pragma unroll 4
+  for (int i = threadIdx.x; i < width / 4; i += kDecodeThreads) {
+    const uint2 raw = in[i];
+    m = __vmaxu2(m, __vmaxu2(raw.x & 0x7fff7fffu, raw.y & 0x7fff7fffu));
+  }
+  m = __reduce_max_sync(0xffffffffu, max(m & 0xffffu, m >> 16));
+  if (lane == 0) largest[warp] = m;
+  __syncthreads();
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) m = __vmaxu2(m, __shfl_xor_sync(0xffffffffu, m, o));
+  for (int w = 0; w < kDecodeWarps; ++w) m = max(m, largest[w]);
   // exponent of the largest, kept where both powers of two are normal numbers
-  const int e = min(max((int)(max(m & 0xffffu, m >> 16) >> 7), 27), 254);
+  const int e = min(max((int)(m >> 7), 27), 254);
   const float inverse = __int_as_float((268 - e) << 23);  // largest / s in [2^14, 2^15)
-  const __nv_bfloat162* pairs = reinterpret_cast<const __nv_bfloat162*>(&raw);
-  const float2 a = __bfloat1622float2(pairs[0]), b = __bfloat1622float2(pairs[1]);
-  const __half2 first = __floats2half2_rn(a.x * inverse, a.y * inverse);
-  const __half2 second = __floats2half2_rn(b.x * inverse, b.y * inverse);
-  out = make_uint2(*reinterpret_cast<const uint32_t*>(&first), *reinterpret_cast<const uint32_t*>(&second));
+#pragma unroll 4
+  for (int i = threadIdx.x; i < width / 4; i += kDecodeThreads) {
+    const uint2 raw = in[i];
+    const __nv_bfloat162* pairs = reinterpret_cast<const __nv_bfloat162*>(&raw);
+    const float2 a = __bfloat1622float2(pairs[0]), b = __bfloat1622float2(pairs[1]);
+    const __half2 first = __floats2half2_rn(a.x * inverse, a.y * inverse);
+    const __half2 second = __floats2half2_rn(b.x * inverse, b.y * inverse);
+    reinterpret_cast<uint2*>(to)[i] =
+        make_uint2(*reinterpret_cast<const uint32_t*>(&first), *reinterpret_cast<const uint32_t*>(&second));
+  }
   return __int_as_float((e - 14) << 23);
 }
 
@@ -159,21 +181,18 @@ __device__ __forceinline__ void load_router(const W* row, int k, int width, bool
 template <typename W, int NT>
 __global__ void __launch_bounds__(kDecodeThreads)
 router_logits_kernel(const __nv_bfloat16* __restrict__ x, const W* __restrict__ router, int T, int E, int width,
-                     float* __restrict__ logits, uint8_t* __restrict__ x16, float* __restrict__ x16_scale) {
+                     float* __restrict__ logits, __half* __restrict__ x16, float* __restrict__ x16_scale) {
   __shared__ float partial[kDecodeWarps][NT * 8][16];
   __shared__ float sums[NT * 8][16];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   const int rank = (int)cluster_ctarank();
   const int routers = (E + 15) / 16 * kRouterCluster;
   if ((int)blockIdx.x >= routers) {  // the clusters behind the router's scale the tokens for the E4M3 products
-    const int blocks = width / 128;
-    const int warps = ((int)gridDim.x - routers) * kDecodeWarps;
-    for (int i = ((int)blockIdx.x - routers) * kDecodeWarps + warp; i < T * blocks; i += warps) {
-      uint2 scaled;
-      const float scale = scale_block(reinterpret_cast<const uint2*>(x)[(long long)i * 32 + lane], scaled);
-      reinterpret_cast<uint2*>(x16)[(long long)i * 32 + lane] = scaled;
-      if (lane == 0) x16_scale[i] = scale;
-    }
+    const int token = (int)blockIdx.x - routers;
+    if (token >= T) return;
+    const float scale = scale_row(x + (long long)token * width, width, x16 + (long long)token * width,
+                                  reinterpret_cast<uint32_t*>(&sums[0][0]));
+    if (threadIdx.x == 0) x16_scale[token] = scale;
     return;
   }
   const int e0 = (blockIdx.x / kRouterCluster) * 16;
@@ -241,12 +260,12 @@ struct DecodeParams {
   const uint8_t *w13, *w2;  // E4M3 or bf16
   const float *w13_scale, *w2_scale;
   const uint8_t *shared_w13, *shared_w2;  // bf16, or null
-  const uint8_t* x16;                     // x against E4M3 weights: [T, D / 128, 256]
-  const float* x16_scale;               // [T, D / 128]
+  const __half* x16;                      // x against E4M3 weights: [T, D], and
+  const float* x16_scale;                 // its powers of two
   __nv_bfloat16* act;                     // [T * K, F] in expert order
   __nv_bfloat16* act_shared;              // [T, shared_inner]
-  uint8_t* act16;                         // act against E4M3 weights: [T * K, F / 128, 256]
-  float* act16_scale;                     // [T * K, F / 128]
+  __half* act16;                          // act against E4M3 weights: [T * K, F]
+  float* act16_scale;
   float* y;                               // [T * K (+ T), D] in expert order, the shared expert's last
   int* row_of;                            // [T * K] row of each assignment
   __nv_bfloat16* out;
@@ -267,16 +286,18 @@ struct Lists {
   int* begin;          // [experts with tokens + 1] first row of each
   uint16_t* expert;    // [experts with tokens]
   uint8_t* tokens;     // [T * K]
+  float* scale;        // [T * K] UP, E4M3: the power of two of each row's token
   int* scratch;        // [E + 64]
   uint16_t* rank;      // [T * K]
   __host__ __device__ static int bytes(int T, int E, int K) {
     const int R = T * K, most = E < R ? E : R;
-    return 4 * (most + 1) + 4 * (E + 64) + 2 * (most + R) + R + 64;
+    return 4 * (most + 1) + 4 * R + 4 * (E + 64) + 2 * (most + R) + R + 64;
   }
   __device__ void place(uint8_t* base, int T, int E, int K) {
     const int R = T * K, most = E < R ? E : R;
     begin = reinterpret_cast<int*>(base);
-    scratch = begin + most + 1;
+    scale = reinterpret_cast<float*>(begin + most + 1);
+    scratch = reinterpret_cast<int*>(scale + R);
     expert = reinterpret_cast<uint16_t*>(scratch + E + 64);
     rank = expert + most;
     tokens = reinterpret_cast<uint8_t*>(rank + R);
@@ -285,7 +306,7 @@ struct Lists {
 
 // Rows by expert, in token order inside one; returns the number of experts with tokens.
 __device__ __forceinline__ int build_lists(const Lists& l, const int* __restrict__ ids, int T, int E, int K,
-                                           int* __restrict__ row_of) {
+                                           int* __restrict__ row_of, const float* __restrict__ token_scale) {
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, R = T * K;
   int* count = l.scratch;           // per expert: rows, then first row
   int* totals = l.scratch + E;      // per warp
@@ -341,7 +362,9 @@ __device__ __forceinline__ int build_lists(const Lists& l, const int* __restrict
   for (int i = tid; i < R; i += kStreamThreads) {
     const int at_row = count[ids[i]] + l.rank[i];
     if (row_of != nullptr) row_of[i] = at_row;
-    l.tokens[at_row] = (uint8_t)(i / K);
+    const int token = i / K;
+    l.tokens[at_row] = (uint8_t)token;
+    if (token_scale != nullptr) l.scale[at_row] = token_scale[token];
   }
   __syncthreads();
   return active;
@@ -440,14 +463,14 @@ struct Barriers {
 };
 
 // A stage's weights: [K block][row], UP: the piece's gate rows, then its up rows, in whole tiles; rows of 128 bytes.
-// Its tokens: [K block][token], and one scale each beside E4M3 weights; two of the weights' scales for each slab.  Fill
+// Its tokens: [K block][token].  Beside E4M3 weights two scales for each slab.  Fill
 // warp w has stages w, w + 4, ...: its first lane sends for the boxes, all its lanes bring the scales and the tokens'
 // columns.  There are at least as many stages as fill warps: a warp that fills stage s has filled s - 4, so
 // s - 4 - count has been read and a wait for s - count cannot take the phase before that one for it.
 template <bool DOWN>
 __device__ __forceinline__ void keep_full(const DecodeParams& p, const DecodeMaps& maps, const Lists& l, int active,
-                                          uint8_t* stages, uint8_t* token_stages, float* token_scales,
-                                          float* weight_scales, int count, Barriers& bars) {
+                                          uint8_t* stages, uint8_t* token_stages, float* weight_scales,
+                                          int count, Barriers& bars) {
   const int lane = threadIdx.x & 31, turn = (threadIdx.x >> 5) - kMultiplyWarps;
   Stream<DOWN> now(p, l, active);
   int slot = 0, stage = 0;
@@ -508,7 +531,6 @@ __device__ __forceinline__ void keep_full(const DecodeParams& p, const DecodeMap
         }
         __syncwarp();
         uint8_t* b = token_stages + slot * p.b_rows * kTokenBytes;
-        float* scales = token_scales + slot * p.b_rows;
         if (!piece.fp8) {
           for (int i = lane; i < rows * 8; i += 32) {
             const int at = i >> 3, ks = here == 1 ? 0 : at / piece.n, row = at - ks * piece.n;
@@ -520,11 +542,9 @@ __device__ __forceinline__ void keep_full(const DecodeParams& p, const DecodeMap
         } else {
           for (int i = lane; i < rows * 16; i += 32) {
             const int at = i >> 4, ks = here == 1 ? 0 : at / piece.n, row = at - ks * piece.n;
-            const long long from =
-                (long long)(DOWN ? piece.begin + row : l.tokens[piece.begin + row]) * piece.blocks + block0 + ks;
+            const long long from = DOWN ? piece.begin + row : l.tokens[piece.begin + row];
             copy16(b + at * kTokenBytes + (((i & 15) ^ (row & 1)) << 4),
-                   (DOWN ? p.act16 : p.x16) + from * kTokenBytes + (i & 15) * 16, true);
-            if ((i & 15) == 0) copy4(scales + at, (DOWN ? p.act16_scale : p.x16_scale) + from);
+                   (DOWN ? p.act16 : p.x16) + from * inner + (block0 + ks) * 128 + (i & 15) * 8, true);
           }
         }
         copies_arrive(full);
@@ -552,65 +572,67 @@ __device__ __forceinline__ void keep_full(const DecodeParams& p, const DecodeMap
 // Weight rows j and j + 4 of a box go to neighbouring lanes: under the 128-byte swizzle they lie in different banks.
 __device__ __forceinline__ int box_row(int g) { return (g >> 1) + ((g & 1) << 2); }
 
-// acc[4 i + h], acc[4 i + 2 + h] are the sums of token 8 i + 2 t + h for the lane's two weight rows.
+__device__ __forceinline__ uint4 load16(uint32_t shared_address) {
+  uint4 v;
+  asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
+               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+               : "r"(shared_address));
+  return v;
+}
+
+// `a`: this lane's first 16 bytes of the slab, the other eight rows `high` bytes further; `b` + token[i]: its first 16 bytes
+// of tile i of the tokens.  acc[4 i + h], acc[4 i + 2 + h] are the sums of token 8 i + 2 t + h for the lane's two weight
+// rows.
 template <int MOST>
-__device__ __forceinline__ void multiply_e4m3(const uint8_t* low, int high, float2 s, const uint8_t* b,
-                                              const float* scales, int n, float (&acc)[MOST * 4]) {
-  const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3, row = box_row(g);
-  const uint8_t* rows = low + row * 128;  // the other eight rows are `high` bytes further
+__device__ __forceinline__ void multiply_e4m3(uint32_t a_at, int high, float2 s, uint32_t b_at, const uint32_t (&token)[MOST],
+                                              int n, float (&acc)[MOST * 4]) {
+  uint32_t a[8][4];
 #pragma unroll
   for (int segment = 0; segment < 2; ++segment) {
-    const int at = ((segment * 4 + t) ^ row) << 4;
-    const uint4 lo = *reinterpret_cast<const uint4*>(rows + at);
-    const uint4 hi = *reinterpret_cast<const uint4*>(rows + high + at);
-    uint32_t a[4][4];
-    widen(lo.x, a[0][0], a[0][2]), widen(hi.x, a[0][1], a[0][3]);
-    widen(lo.y, a[1][0], a[1][2]), widen(hi.y, a[1][1], a[1][3]);
-    widen(lo.z, a[2][0], a[2][2]), widen(hi.z, a[2][1], a[2][3]);
-    widen(lo.w, a[3][0], a[3][2]), widen(hi.w, a[3][1], a[3][3]);
+    const uint4 lo = load16(a_at ^ (segment * 64)), hi = load16((a_at ^ (segment * 64)) + high);
+    const int j = segment * 4;
+    widen(lo.x, a[j][0], a[j][2]), widen(hi.x, a[j][1], a[j][3]);
+    widen(lo.y, a[j + 1][0], a[j + 1][2]), widen(hi.y, a[j + 1][1], a[j + 1][3]);
+    widen(lo.z, a[j + 2][0], a[j + 2][2]), widen(hi.z, a[j + 2][1], a[j + 2][3]);
+    widen(lo.w, a[j + 3][0], a[j + 3][2]), widen(hi.w, a[j + 3][1], a[j + 3][3]);
+  }
 #pragma unroll
-    for (int i = 0; i < MOST; ++i) {
-      if (i * 8 < n) {
-        const int token = min(i * 8 + g, n - 1), chunk = (segment * 8 + 2 * t) ^ (token & 1);
-        const uint4 v0 = *reinterpret_cast<const uint4*>(b + token * kTokenBytes + (chunk << 4));
-        const uint4 v1 = *reinterpret_cast<const uint4*>(b + token * kTokenBytes + ((chunk ^ 1) << 4));
-        float c[4] = {0.f, 0.f, 0.f, 0.f};
-        mma_f16(c, a[0][0], a[0][1], a[0][2], a[0][3], v0.x, v0.y);
-        mma_f16(c, a[1][0], a[1][1], a[1][2], a[1][3], v0.z, v0.w);
-        mma_f16(c, a[2][0], a[2][1], a[2][2], a[2][3], v1.x, v1.y);
-        mma_f16(c, a[3][0], a[3][1], a[3][2], a[3][3], v1.z, v1.w);
-        const float t0 = scales[min(i * 8 + 2 * t, n - 1)], t1 = scales[min(i * 8 + 2 * t + 1, n - 1)];
-        acc[4 * i] = fmaf(c[0], s.x * t0, acc[4 * i]);
-        acc[4 * i + 1] = fmaf(c[1], s.x * t1, acc[4 * i + 1]);
-        acc[4 * i + 2] = fmaf(c[2], s.y * t0, acc[4 * i + 2]);
-        acc[4 * i + 3] = fmaf(c[3], s.y * t1, acc[4 * i + 3]);
-      }
+  for (int i = 0; i < MOST; ++i) {
+    if (i * 8 < n) {
+      const uint32_t at = b_at + token[i];
+      float c[4];
+      const uint4 v0 = load16(at), v1 = load16(at ^ 16);
+      mma_f16_from_zero(c, a[0], v0.x, v0.y);
+      mma_f16(c, a[1], v0.z, v0.w);
+      mma_f16(c, a[2], v1.x, v1.y);
+      mma_f16(c, a[3], v1.z, v1.w);
+      const uint4 v2 = load16(at + 128), v3 = load16((at ^ 16) + 128);
+      mma_f16(c, a[4], v2.x, v2.y);
+      mma_f16(c, a[5], v2.z, v2.w);
+      mma_f16(c, a[6], v3.x, v3.y);
+      mma_f16(c, a[7], v3.z, v3.w);
+      acc[4 * i] = fmaf(c[0], s.x, acc[4 * i]);
+      acc[4 * i + 1] = fmaf(c[1], s.x, acc[4 * i + 1]);
+      acc[4 * i + 2] = fmaf(c[2], s.y, acc[4 * i + 2]);
+      acc[4 * i + 3] = fmaf(c[3], s.y, acc[4 * i + 3]);
     }
   }
 }
 
 // The same on bf16 weights.
 template <int MOST>
-__device__ __forceinline__ void multiply_bf16(const uint8_t* low, int high, const uint8_t* b, int n,
+__device__ __forceinline__ void multiply_bf16(uint32_t a_at, int high, uint32_t b_at, const uint32_t (&token)[MOST], int n,
                                               float (&acc)[MOST * 4]) {
-  const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3, row = box_row(g);
-  uint4 lo[2], hi[2];
-#pragma unroll
-  for (int segment = 0; segment < 2; ++segment) {
-    const uint8_t* at = low + row * 128 + (((segment * 4 + t) ^ row) << 4);
-    lo[segment] = *reinterpret_cast<const uint4*>(at);
-    hi[segment] = *reinterpret_cast<const uint4*>(at + high);
-  }
+  const uint4 l0 = load16(a_at), h0 = load16(a_at + high), l1 = load16(a_at ^ 64), h1 = load16((a_at ^ 64) + high);
 #pragma unroll
   for (int i = 0; i < MOST; ++i) {
     if (i * 8 < n) {
-      const uint8_t* token = b + min(i * 8 + g, n - 1) * kTokenPitchBf16 + t * 16;
-      const uint4 v0 = *reinterpret_cast<const uint4*>(token), v1 = *reinterpret_cast<const uint4*>(token + 64);
+      const uint4 v0 = load16(b_at + token[i]), v1 = load16(b_at + token[i] + 64);
       float(&c)[4] = *reinterpret_cast<float(*)[4]>(&acc[4 * i]);
-      mma_bf16(c, lo[0].x, hi[0].x, lo[0].y, hi[0].y, v0.x, v0.y);
-      mma_bf16(c, lo[0].z, hi[0].z, lo[0].w, hi[0].w, v0.z, v0.w);
-      mma_bf16(c, lo[1].x, hi[1].x, lo[1].y, hi[1].y, v1.x, v1.y);
-      mma_bf16(c, lo[1].z, hi[1].z, lo[1].w, hi[1].w, v1.z, v1.w);
+      mma_bf16(c, l0.x, h0.x, l0.y, h0.y, v0.x, v0.y);
+      mma_bf16(c, l0.z, h0.z, l0.w, h0.w, v0.z, v0.w);
+      mma_bf16(c, l1.x, h1.x, l1.y, h1.y, v1.x, v1.y);
+      mma_bf16(c, l1.z, h1.z, l1.w, h1.w, v1.z, v1.w);
     }
   }
 }
@@ -631,8 +653,7 @@ stream_kernel(const DecodeParams p, const __grid_constant__ DecodeMaps maps, int
   __shared__ Barriers bars;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
   uint8_t* token_stages = shared_memory + stages * kStageA;
-  float* token_scales = reinterpret_cast<float*>(token_stages + stages * p.b_rows * kTokenBytes);
-  float* weight_scales = token_scales + stages * p.b_rows;
+  float* weight_scales = reinterpret_cast<float*>(token_stages + stages * p.b_rows * kTokenBytes);
   float* meet = weight_scales + stages * kStageScales;  // [slab][value][lane]
   __shared__ Lists l;  // (in shared memory: its pointers took ten registers)
   if (tid == 0) {
@@ -647,9 +668,10 @@ stream_kernel(const DecodeParams p, const __grid_constant__ DecodeMaps maps, int
     tma_prefetch_desc(&maps.flat);
   }
   __syncthreads();
-  const int active = build_lists(l, p.ids, p.T, p.E, p.K, !DOWN && blockIdx.x == 0 ? p.row_of : nullptr);
+  const int active = build_lists(l, p.ids, p.T, p.E, p.K, !DOWN && blockIdx.x == 0 ? p.row_of : nullptr,
+                                 !DOWN && p.fp8 ? p.x16_scale : nullptr);
   if (warp >= kMultiplyWarps) {
-    keep_full<DOWN>(p, maps, l, active, shared_memory, token_stages, token_scales, weight_scales, stages, bars);
+    keep_full<DOWN>(p, maps, l, active, shared_memory, token_stages, weight_scales, stages, bars);
     return;
   }
 
@@ -666,22 +688,32 @@ stream_kernel(const DecodeParams p, const __grid_constant__ DecodeMaps maps, int
     const bool mine = ks < ks_count && rt * kTile < piece.count;
     // this lane's two weight rows are `column` and, 8 further (DOWN) or the up row of the same column (UP)
     const int column = rt * kTile + box_row(g);
-    const int low = (ks << piece.rt_log) * kSlab + rt * (DOWN ? 2048 : 1024), high = DOWN ? 1024 : 1024 << piece.rt_log;
-    const int first_token = ks * piece.n;
+    const int high = DOWN ? 1024 : 1024 << piece.rt_log;
+    const uint32_t a_first = smem_u32(shared_memory) + (ks << piece.rt_log) * kSlab + rt * (DOWN ? 2048 : 1024) +
+                             box_row(g) * 128 + ((t ^ box_row(g)) << 4);
+    const int pitch = piece.fp8 ? kTokenBytes : kTokenPitchBf16;
+    const uint32_t b_first = smem_u32(token_stages) + ks * piece.n * pitch;
+    uint32_t token[MOST];
+#pragma unroll
+    for (int i = 0; i < MOST; ++i) {
+      const int j = min(i * 8 + g, piece.n - 1);
+      token[i] = j * pitch + (piece.fp8 ? ((2 * t) ^ (j & 1)) << 4 : t << 4);
+    }
     float acc[MOST * 4];
 #pragma unroll
     for (int i = 0; i < MOST * 4; ++i) acc[i] = 0.f;
+    const int n = piece.n, blocks = mine ? piece.blocks : 0;
+    const bool fp8 = piece.fp8;
     int block = ks;
-    for (int step = 0; step < piece.steps; ++step, block += ks_count) {
+    for (int step = piece.steps; step > 0; --step, block += ks_count) {
       if (!dead) dead = !wait_stage(&bars.full[slot], phase, &bars.abort, p.status, 72);
-      if (mine && block < piece.blocks) {
-        const uint8_t* a = shared_memory + slot * kStageA + low;
-        const uint8_t* b = token_stages + slot * p.b_rows * kTokenBytes;
-        if (piece.fp8)
-          multiply_e4m3<MOST>(a, high, reinterpret_cast<const float2*>(weight_scales + slot * kStageScales)[warp],
-                              b + first_token * kTokenBytes, token_scales + slot * p.b_rows + first_token, piece.n, acc);
+      if (block < blocks) {
+        const uint32_t a = a_first + slot * kStageA, b = b_first + slot * p.b_rows * kTokenBytes;
+        if (fp8)
+          multiply_e4m3<MOST>(a, high, reinterpret_cast<const float2*>(weight_scales + slot * kStageScales)[warp], b, token,
+                              n, acc);
         else
-          multiply_bf16<MOST>(a, high, b + first_token * kTokenPitchBf16, piece.n, acc);
+          multiply_bf16<MOST>(a, high, b, token, n, acc);
       }
       __syncwarp();
       if (lane == 0) mbar_arrive(&bars.empty[slot]);
@@ -712,8 +744,12 @@ stream_kernel(const DecodeParams p, const __grid_constant__ DecodeMaps maps, int
 #pragma unroll
       for (int q = 0; q < MOST * 2; ++q) {
         const int j = (q >> 1) * 8 + 2 * t + (q & 1);
-        const float first = acc[(q >> 1) * 4 + (q & 1)], second = acc[(q >> 1) * 4 + 2 + (q & 1)];
+        float first = acc[(q >> 1) * 4 + (q & 1)], second = acc[(q >> 1) * 4 + 2 + (q & 1)];
         if (j < piece.n) {
+          if (!DOWN && piece.fp8) {
+            const float scale = l.scale[piece.begin + j];
+            first *= scale, second *= scale;
+          }
           const long long at = (long long)(piece.begin + j) * width + piece.first + column;
           if (DOWN) {
             float* to = p.y + (is_shared ? (long long)p.T * p.K * p.D : 0) + at;
@@ -728,16 +764,13 @@ stream_kernel(const DecodeParams p, const __grid_constant__ DecodeMaps maps, int
   }
 }
 
-// act [rows, F] for the E4M3 down product: f16 with a power of two per 128 columns, a warp to a block.
+// act [rows, F] for the E4M3 down product, a block to a row.
 __global__ void __launch_bounds__(kDecodeThreads)
-scale_act_kernel(const __nv_bfloat16* __restrict__ act, int blocks, uint8_t* __restrict__ act16,
-                 float* __restrict__ act16_scale) {
-  const int i = blockIdx.x * kDecodeWarps + (threadIdx.x >> 5), lane = threadIdx.x & 31;
-  if (i >= blocks) return;
-  uint2 scaled;
-  const float scale = scale_block(reinterpret_cast<const uint2*>(act)[(long long)i * 32 + lane], scaled);
-  reinterpret_cast<uint2*>(act16)[(long long)i * 32 + lane] = scaled;
-  if (lane == 0) act16_scale[i] = scale;
+scale_act_kernel(const __nv_bfloat16* __restrict__ act, int F, __half* __restrict__ act16, float* __restrict__ act16_scale) {
+  __shared__ uint32_t largest[kDecodeWarps];
+  const long long at = (long long)blockIdx.x * F;
+  const float scale = scale_row(act + at, F, act16 + at, largest);
+  if (threadIdx.x == 0) act16_scale[blockIdx.x] = scale;
 }
 
 // out[t] = residual[t] + sum_k w[t,k] y[row_of[t,k]] (+ the shared expert's row of t): fp32, k ascending, one rounding.
@@ -751,8 +784,10 @@ join_kernel(const DecodeParams p) {
 #pragma unroll
   for (int i = 0; i < 4; ++i) v[i] = __bfloat162float(p.residual[at + i]);
   for (int k = 0; k < p.K; ++k) {
-    const float w = p.route_weights[t * p.K + k];
-    const float4 y = *reinterpret_cast<const float4*>(p.y + (long long)p.row_of[t * p.K + k] * p.D + c);
+    const int row = p.row_of[t * p.K + k];
+    float w = p.route_weights[t * p.K + k];
+    if (p.fp8) w *= p.act16_scale[row];  // (a power of two)
+    const float4 y = *reinterpret_cast<const float4*>(p.y + (long long)row * p.D + c);
     v[0] = fmaf(w, y.x, v[0]), v[1] = fmaf(w, y.y, v[1]), v[2] = fmaf(w, y.z, v[2]), v[3] = fmaf(w, y.w, v[3]);
   }
   if (p.shared_inner > 0) {
@@ -769,12 +804,12 @@ struct DecodeWorkspace {
     const auto up = [](long long n) { return (n + 255) / 256 * 256; };
     logits = 0;
     x16 = up(4 * T * E);
-    x16_scale = x16 + up(T * (D / 128) * kTokenBytes);
-    act = x16_scale + up(4 * T * (D / 128));
+    x16_scale = x16 + up(2 * T * D);
+    act = x16_scale + up(4 * T);
     act_shared = act + up(2 * T * K * F);
     act16 = act_shared + up(2 * T * shared_inner);
-    act16_scale = act16 + up(T * K * (F / 128) * kTokenBytes);
-    y = act16_scale + up(4 * T * K * (F / 128));
+    act16_scale = act16 + up(2 * T * K * F);
+    y = act16_scale + up(4 * T * K);
     row_of = y + up(4 * (T * K + (shared_inner > 0 ? T : 0)) * D);
     bytes = row_of + up(4 * T * K);
   }
@@ -791,10 +826,10 @@ static int decode_sizes(long long tokens, int width, int inner, int experts, int
 }
 
 template <typename W>
-static int launch_router(const b200moe_decode_args* a, float* logits, uint8_t* x16, float* x16_scale,
+static int launch_router(const b200moe_decode_args* a, float* logits, __half* x16, float* x16_scale,
                          cudaStream_t s) {
   cudaLaunchConfig_t config = {};
-  const int scaling = x16 != nullptr ? ((int)a->tokens + 15) / 16 : 0;  // clusters, a warp for each 128 columns of 16 tokens
+  const int scaling = x16 != nullptr ? ((int)a->tokens + kRouterCluster - 1) / kRouterCluster : 0;  // a block to a token
   config.gridDim = dim3((unsigned)(((a->experts + 15) / 16 + scaling) * kRouterCluster));
   config.blockDim = dim3(kDecodeThreads);
   config.stream = s;
@@ -822,7 +857,7 @@ static int encode_weights(CUtensorMap* map, const void* base, bool fp8, long lon
 
 template <bool DOWN, int MOST>
 static int launch_stream(const DecodeParams& p, const DecodeMaps& maps, cudaStream_t s) {
-  const int stage = kStageA + p.b_rows * (kTokenBytes + 4) + kStageScales * 4;
+  const int stage = kStageA + p.b_rows * kTokenBytes + kStageScales * 4;
   const int rest = meet_bytes(p.T) + Lists::bytes(p.T, p.E, p.K);
   int stages = (225 * 1024 - rest) / stage;
   if (stages > kMaxStages) stages = kMaxStages;
@@ -842,9 +877,7 @@ static int launch_streams(const DecodeParams& p, const DecodeMaps& up, const Dec
   int code = launch_stream<false, MOST>(p, up, s);
   if (code != B200MOE_OK) return code;
   if (p.fp8) {
-    const int blocks = p.T * p.K * (p.F / 128);
-    scale_act_kernel<<<(blocks + kDecodeWarps - 1) / kDecodeWarps, kDecodeThreads, 0, s>>>(p.act, blocks, p.act16,
-                                                                                          p.act16_scale);
+    scale_act_kernel<<<p.T * p.K, kDecodeThreads, 0, s>>>(p.act, p.F, p.act16, p.act16_scale);
   }
   code = launch_stream<true, MOST>(p, down, s);
   if (code != B200MOE_OK) return code;
@@ -904,7 +937,7 @@ extern "C" int b200moe_decode(const b200moe_decode_args* a, void* stream) {
   char* base = reinterpret_cast<char*>(a->workspace);
   float* logits = reinterpret_cast<float*>(base + w.logits);
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
-  uint8_t* x16 = fp8 ? reinterpret_cast<uint8_t*>(base + w.x16) : nullptr;
+  __half* x16 = fp8 ? reinterpret_cast<__half*>(base + w.x16) : nullptr;
   float* x16_scale = reinterpret_cast<float*>(base + w.x16_scale);
   code = a->router_is_fp32 ? launch_router<float>(a, logits, x16, x16_scale, s)
                            : launch_router<__nv_bfloat16>(a, logits, x16, x16_scale, s);
@@ -926,7 +959,7 @@ extern "C" int b200moe_decode(const b200moe_decode_args* a, void* stream) {
   p.x16 = x16;
   p.x16_scale = x16_scale;
   p.act = reinterpret_cast<__nv_bfloat16*>(base + w.act);
-  p.act16 = reinterpret_cast<uint8_t*>(base + w.act16);
+  p.act16 = reinterpret_cast<__half*>(base + w.act16);
   p.act16_scale = reinterpret_cast<float*>(base + w.act16_scale);
   p.y = reinterpret_cast<float*>(base + w.y);
   p.row_of = reinterpret_cast<int*>(base + w.row_of);
