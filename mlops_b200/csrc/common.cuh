@@ -37,6 +37,13 @@ __device__ __forceinline__ uint32_t smem_u32(const void* p) {
   return (uint32_t)__cvta_generic_to_shared(p);
 }
 
+// A kernel launched as a dependent (launch_dependent on the host) may start before the one in front of it in the
+// stream has finished: it waits here before it touches what that one writes.  Without the launch attribute
+// the wait returns at once.
+__device__ __forceinline__ void dependency_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+// Lets the dependent kernel start once every block of this one has called it (or has finished).
+__device__ __forceinline__ void dependency_release() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+
 // ----------------------------------------------------------------------------
 // mbarrier
 // ----------------------------------------------------------------------------

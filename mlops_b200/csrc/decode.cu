@@ -26,6 +26,8 @@
 // a weight row the tensor rate is not what bounds this.  Sums are fp32; act is rounded to bf16 once, as the operand of the
 // second product (the grouped layer rounds it likewise), and the output once.  Every sum has a fixed order: no
 // atomics.
+#include <atomic>
+
 #include "common.cuh"
 #include "host_util.h"
 #include "../../include/b200moe.h"
@@ -186,6 +188,7 @@ router_logits_kernel(const __nv_bfloat16* __restrict__ x, const W* __restrict__ 
   __shared__ float sums[NT * 8][16];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   const int rank = (int)cluster_ctarank();
+  dependency_release();
   const int routers = (E + 15) / 16 * kRouterCluster;
   if ((int)blockIdx.x >= routers) {  // the clusters behind the router's scale the tokens for the E4M3 products
     const int token = (int)blockIdx.x - routers;
@@ -462,6 +465,25 @@ struct Barriers {
   int abort;
 };
 
+// Asks for the first rows this CTA's part of the down product will read: HBM would idle while the last sums of the up
+// product are formed, act is scaled and the next kernel starts.
+constexpr long long kPrefetchBytes = 256 << 10;
+__device__ __forceinline__ void prefetch_down(const DecodeParams& p, const Lists& l, int active) {
+  Stream<true> now(p, l, active);
+  const long long pitch = (long long)p.F * (p.fp8 ? 1 : 2);
+  int last = -1;
+  for (long long left = kPrefetchBytes; left > 0 && now.next() && now.piece.index < active;) {
+    if (now.piece.index == last && now.piece.begin > l.begin[last]) continue;  // another pass over the same rows
+    last = now.piece.index;
+    const uint8_t* from = p.w2 + ((long long)l.expert[last] * p.D + now.piece.first) * pitch;
+    const long long bytes = min(left, now.piece.count * pitch);
+    for (long long at = 0; at < bytes; at += 16384)
+      asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(from + at), "r"((uint32_t)min(16384LL, bytes - at))
+                   : "memory");
+    left -= bytes;
+  }
+}
+
 // A stage's weights: [K block][row], UP: the piece's gate rows, then its up rows, in whole tiles; rows of 128 bytes.
 // Its tokens: [K block][token].  Beside E4M3 weights two scales for each slab.  Fill
 // warp w has stages w, w + 4, ...: its first lane sends for the boxes, all its lanes bring the scales and the tokens'
@@ -530,6 +552,7 @@ __device__ __forceinline__ void keep_full(const DecodeParams& p, const DecodeMap
           }
         }
         __syncwarp();
+        if (DOWN && stage < kFillWarps) dependency_wait();  // the first weights are on their way, act must be there
         uint8_t* b = token_stages + slot * p.b_rows * kTokenBytes;
         if (!piece.fp8) {
           for (int i = lane; i < rows * 8; i += 32) {
@@ -555,6 +578,7 @@ __device__ __forceinline__ void keep_full(const DecodeParams& p, const DecodeMap
       }
     }
   }
+  if (!DOWN && turn == 0 && lane == 0) prefetch_down(p, l, active);
   if (dead) {  // nothing of this warp's may still be on its way when it leaves
     volatile int go_on = 0;
     for (int i = 1; i <= min(stage, count); ++i) {
@@ -668,6 +692,10 @@ stream_kernel(const DecodeParams p, const __grid_constant__ DecodeMaps maps, int
     tma_prefetch_desc(&maps.flat);
   }
   __syncthreads();
+  // UP starts from the routing; when its blocks have seen that finished they let the next kernels start, so that
+  // DOWN finds the routing finished and waits for act alone (keep_full)
+  if (!DOWN) dependency_wait();
+  dependency_release();
   const int active = build_lists(l, p.ids, p.T, p.E, p.K, !DOWN && blockIdx.x == 0 ? p.row_of : nullptr,
                                  !DOWN && p.fp8 ? p.x16_scale : nullptr);
   if (warp >= kMultiplyWarps) {
@@ -769,6 +797,8 @@ __global__ void __launch_bounds__(kDecodeThreads)
 scale_act_kernel(const __nv_bfloat16* __restrict__ act, int F, __half* __restrict__ act16, float* __restrict__ act16_scale) {
   __shared__ uint32_t largest[kDecodeWarps];
   const long long at = (long long)blockIdx.x * F;
+  dependency_release();
+  dependency_wait();
   const float scale = scale_row(act + at, F, act16 + at, largest);
   if (threadIdx.x == 0) act16_scale[blockIdx.x] = scale;
 }
@@ -778,6 +808,7 @@ scale_act_kernel(const __nv_bfloat16* __restrict__ act, int F, __half* __restric
 __global__ void __launch_bounds__(kDecodeThreads)
 join_kernel(const DecodeParams p) {
   const int t = blockIdx.y, c = (blockIdx.x * kDecodeThreads + threadIdx.x) * 4;
+  dependency_wait();
   if (c >= p.D) return;
   const long long at = (long long)t * p.D + c;
   float v[4];
@@ -864,12 +895,17 @@ static int launch_stream(const DecodeParams& p, const DecodeMaps& maps, cudaStre
   if (stages < kFillWarps) return B200MOE_ERR_LIMIT;
   const int bytes = stages * stage + rest;
   const auto kernel = stream_kernel<DOWN, MOST>;
-  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) != cudaSuccess) {
-    cudaGetLastError();
-    return B200MOE_ERR_LAUNCH;
+  static std::atomic<unsigned long long> allowed{0};  // devices on which the kernel may have that much shared memory
+  int device = 0;
+  if (cudaGetDevice(&device) != cudaSuccess || device >= 64) return B200MOE_ERR_LAUNCH;
+  if (!((allowed.load(std::memory_order_relaxed) >> device) & 1)) {
+    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 225 * 1024) != cudaSuccess) {
+      cudaGetLastError();
+      return B200MOE_ERR_LAUNCH;
+    }
+    allowed.fetch_or(1ull << device, std::memory_order_relaxed);
   }
-  kernel<<<sm_count(), kStreamThreads, bytes, s>>>(p, maps, stages);
-  return launch_status();
+  return launch_dependent(kernel, sm_count(), kStreamThreads, bytes, s, true, p, maps, stages);
 }
 
 template <int MOST>
@@ -877,12 +913,13 @@ static int launch_streams(const DecodeParams& p, const DecodeMaps& up, const Dec
   int code = launch_stream<false, MOST>(p, up, s);
   if (code != B200MOE_OK) return code;
   if (p.fp8) {
-    scale_act_kernel<<<p.T * p.K, kDecodeThreads, 0, s>>>(p.act, p.F, p.act16, p.act16_scale);
+    code = launch_dependent(scale_act_kernel, p.T * p.K, kDecodeThreads, 0, s, true, p.act, p.F, p.act16, p.act16_scale);
+    if (code != B200MOE_OK) return code;
   }
   code = launch_stream<true, MOST>(p, down, s);
   if (code != B200MOE_OK) return code;
-  join_kernel<<<dim3((p.D / 4 + kDecodeThreads - 1) / kDecodeThreads, p.T), kDecodeThreads, 0, s>>>(p);
-  return launch_status();
+  return launch_dependent(join_kernel, dim3((p.D / 4 + kDecodeThreads - 1) / kDecodeThreads, p.T), kDecodeThreads, 0, s,
+                          true, p);
 }
 
 }  // namespace b200
@@ -942,8 +979,8 @@ extern "C" int b200moe_decode(const b200moe_decode_args* a, void* stream) {
   code = a->router_is_fp32 ? launch_router<float>(a, logits, x16, x16_scale, s)
                            : launch_router<__nv_bfloat16>(a, logits, x16, x16_scale, s);
   if (code != B200MOE_OK) return code;
-  code = b200moe_route_topk(logits, a->experts, (int)a->tokens, a->experts, a->top_k, a->mode, a->bias, a->n_group,
-                            a->topk_group, a->routed_scaling, a->route_weights, a->ids, stream);
+  code = launch_route_topk(logits, a->experts, (int)a->tokens, a->experts, a->top_k, a->mode, a->bias, a->n_group,
+                           a->topk_group, a->routed_scaling, a->route_weights, a->ids, true, s);
   if (code != B200MOE_OK) return code;
   DecodeParams p = {};
   p.x = reinterpret_cast<const __nv_bfloat16*>(a->x);

@@ -42,6 +42,29 @@ int launch_routing_gradient(const float* logits, long long ld, long long tokens,
                             const float* grad_aux, const float* frequency, float aux_scale,
                             const float* grad_probability_sum, float* grad_logits, long long ldg, void* high,
                             void* low, cudaStream_t s);
+// b200moe_route_topk; `dependent`: launched as a dependent of the kernel in front of it.
+int launch_route_topk(const float* logits, long long ld, int tokens, int experts, int top_k, int mode, const float* bias,
+                      int n_group, int topk_group, float routed_scaling, float* weights, int32_t* ids, bool dependent,
+                      cudaStream_t s);
+// Launches `kernel`; `dependent`: it may start before the kernel in front of it in the stream has finished, and waits
+// for that one itself (dependency_wait).
+template <typename... Params, typename... Args>
+inline int launch_dependent(void (*kernel)(Params...), dim3 grid, dim3 block, size_t shared, cudaStream_t s, bool dependent,
+                            Args... args) {
+  cudaLaunchConfig_t config = {};
+  config.gridDim = grid;
+  config.blockDim = block;
+  config.dynamicSmemBytes = shared;
+  config.stream = s;
+  cudaLaunchAttribute attribute;
+  attribute.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attribute.val.programmaticStreamSerializationAllowed = 1;
+  config.attrs = &attribute;
+  config.numAttrs = dependent ? 1 : 0;
+  if (cudaLaunchKernelEx(&config, kernel, static_cast<Params>(args)...) == cudaSuccess) return B200MOE_OK;
+  cudaGetLastError();
+  return B200MOE_ERR_LAUNCH;
+}
 int sm_count_device();      // SM count of the current device (cached per device)
 int sm_count();             // CTAs a persistent kernel may launch: the SM count, or the limit below
 void set_cta_limit(int n);  // n > 0: persistent kernels launch at most n CTAs; 0: no limit

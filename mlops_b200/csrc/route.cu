@@ -50,6 +50,8 @@ route_topk_kernel(const float* __restrict__ logits, long long ld, int T, int E, 
                   float* __restrict__ weights, int* __restrict__ ids) {
   const int lane = threadIdx.x & 31;
   const int t = blockIdx.x * kRouteWarps + (threadIdx.x >> 5);
+  dependency_release();
+  dependency_wait();
   if (t >= T) return;
   const float NEG_INF = __int_as_float(0xff800000);
 
@@ -389,9 +391,9 @@ sort_small_kernel(const int* __restrict__ ids, int R, int E, int* __restrict__ o
 
 using namespace b200;
 
-extern "C" int b200moe_route_topk(const float* logits, long long ld, int tokens, int experts, int top_k,
-                                  int mode, const float* bias, int n_group, int topk_group,
-                                  float routed_scaling, float* weights, int32_t* ids, void* stream) {
+int b200::launch_route_topk(const float* logits, long long ld, int tokens, int experts, int top_k, int mode,
+                            const float* bias, int n_group, int topk_group, float routed_scaling, float* weights,
+                            int32_t* ids, bool dependent, cudaStream_t s) {
   if (!logits || !weights || !ids) return B200MOE_ERR_ARG;
   if (tokens < 0 || experts <= 0 || top_k <= 0 || top_k > experts || mode < 0 || mode > 2)
     return B200MOE_ERR_ARG;
@@ -401,21 +403,23 @@ extern "C" int b200moe_route_topk(const float* logits, long long ld, int tokens,
     if (n_group > 32 && topk_group < n_group) return B200MOE_ERR_LIMIT;
   }
   if (tokens == 0) return B200MOE_OK;
-  cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
   const unsigned grid = (unsigned)((tokens + kRouteWarps - 1) / kRouteWarps);
   const int epl = (experts + 31) / 32;
-#define LAUNCH_ROUTE(EPL)                                                                              \
-  route_topk_kernel<EPL><<<grid, kRouteWarps * 32, 0, s>>>(logits, ld, tokens, experts, top_k, mode,   \
-                                                          bias, n_group, topk_group, routed_scaling,   \
-                                                          weights, ids)
-  if (epl <= 1) LAUNCH_ROUTE(1);
-  else if (epl <= 2) LAUNCH_ROUTE(2);
-  else if (epl <= 4) LAUNCH_ROUTE(4);
-  else if (epl <= 8) LAUNCH_ROUTE(8);
-  else if (epl <= 16) LAUNCH_ROUTE(16);
-  else LAUNCH_ROUTE(32);
-#undef LAUNCH_ROUTE
-  return launch_status();
+  const auto kernel = epl <= 1   ? route_topk_kernel<1>
+                      : epl <= 2 ? route_topk_kernel<2>
+                      : epl <= 4 ? route_topk_kernel<4>
+                      : epl <= 8 ? route_topk_kernel<8>
+                      : epl <= 16 ? route_topk_kernel<16>
+                                  : route_topk_kernel<32>;
+  return launch_dependent(kernel, grid, kRouteWarps * 32, 0, s, dependent, logits, ld, tokens, experts, top_k, mode, bias,
+                          n_group, topk_group, routed_scaling, weights, ids);
+}
+
+extern "C" int b200moe_route_topk(const float* logits, long long ld, int tokens, int experts, int top_k,
+                                  int mode, const float* bias, int n_group, int topk_group,
+                                  float routed_scaling, float* weights, int32_t* ids, void* stream) {
+  return launch_route_topk(logits, ld, tokens, experts, top_k, mode, bias, n_group, topk_group, routed_scaling, weights,
+                           ids, false, reinterpret_cast<cudaStream_t>(stream));
 }
 
 extern "C" long long b200moe_sort_assignments_workspace_bytes(long long assignments, int experts) {

@@ -257,14 +257,20 @@ def forward_decode(
     backward pass and no statistics are formed. Activations stay bf16 on block-FP8 weights too
     (`forward_routed` quantises them to E4M3), so the output is the nearer of the two to the weights' exact product.
     `shared = (w13 [2Fs, D], w2 [D, Fs])` (bf16) adds the always-on shared expert."""
-    with torch.no_grad():
-        rows = h2.reshape(-1, h2.shape[-1]).contiguous()
-        bias = None if router_bias is None or router_bias.numel() == 0 else router_bias
-        output, weights, ids = ops.moe_decode(
-            rows, residual.reshape(rows.shape).contiguous(), getattr(router_weight, "_data", router_weight), w13, w2,
-            top_k=top_k, mode=str(routing_mode), bias=bias, n_group=n_group, topk_group=topk_group,
-            routed_scaling=routed_scaling, limit=swiglu_limit, shared=shared)
-        return output.view(h2.shape), weights, ids
+    shape = h2.shape
+    if len(shape) != 2:
+        h2 = h2.reshape(-1, shape[-1])
+    if residual.shape != h2.shape:
+        residual = residual.reshape(h2.shape)
+    if type(router_weight) not in (torch.Tensor, torch.nn.Parameter):
+        router_weight = getattr(router_weight, "_data", router_weight)
+    if router_bias is not None and router_bias.numel() == 0:
+        router_bias = None
+    output, weights, ids = ops.moe_decode(
+        h2.contiguous(), residual.contiguous(), router_weight, w13, w2, top_k=top_k, mode=routing_mode,
+        bias=router_bias, n_group=n_group, topk_group=topk_group, routed_scaling=routed_scaling, limit=swiglu_limit,
+        shared=shared)
+    return output if len(shape) == 2 else output.view(shape), weights, ids
 
 
 def _swiglu(h13, save8, **kwargs):

@@ -105,7 +105,8 @@ def set_gemm_pair(mode: int) -> None:
 
 
 def _stream() -> int:
-    return torch.cuda.current_stream().cuda_stream
+    # (torch.cuda.current_stream() makes a Stream object first: 3 us against 0.5)
+    return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device())
 
 
 def _need_cuda(*tensors) -> torch.device:
