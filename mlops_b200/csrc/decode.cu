@@ -47,6 +47,7 @@ constexpr int kTokenBytes = 256;      // a token's 128 columns beside an E4M3 bl
 constexpr int kTokenPitchBf16 = 192;  // its 64 beside a bf16 block: rows start in different banks
 constexpr int kStageScales = 2 * kStageSlabs;  // of the weights: each slab's first and other eight rows
 constexpr int kMaxStages = 8;
+constexpr int kJoinColumns = 256;
 constexpr int kPassTokens = 32;  // of one expert that a pass over its weights takes; rarely has an expert more
 
 __device__ __forceinline__ void copy16(void* dst, const void* src, bool read) {
@@ -385,35 +386,33 @@ struct Piece {
   bool fp8;
 };
 
+// Their order: UP expert by expert, the shared one last; DOWN the same within each kJoinColumns columns (a block), .
 template <bool DOWN>
 struct Stream {
   const DecodeParams& p;
   const Lists& l;
   const int active;
-  int at, end;  // flat output columns of the experts with tokens, then the shared expert's
-  int waiting;  // tokens of the current expert that need another pass over the same weights
+  int at, end;             // flat output columns
+  int block, block_end;    // the current block and where it ends
+  int waiting;             // tokens of the current expert that need another pass over the same weights
   Piece piece;
 
   // The columns are cut between the CTAs in whole groups of eight, what a flat box of weights holds.
   __device__ Stream(const DecodeParams& params, const Lists& lists, int n_active)
       : p(params), l(lists), active(n_active), waiting(0) {
     const long long b = blockIdx.x, grid = gridDim.x;
-    const long long total = (long long)active * width() + (long long)shared_cost() * shared_width();
+    const long long total = DOWN ? (long long)p.D * (active + shared_cost())
+                                 : (long long)active * p.F + (long long)shared_cost() * p.shared_inner;
     at = (int)(total / 8 * b / grid) * 8;
     end = (int)(total / 8 * (b + 1) / grid) * 8;
   }
-  __device__ int width() const { return DOWN ? p.D : p.F; }
-  __device__ int shared_width() const { return p.shared_inner == 0 ? 0 : DOWN ? p.D : p.shared_inner; }
   // what a column of the shared expert (bf16) costs in columns of the others
   __device__ int shared_cost() const {
-    const int bytes = p.fp8 ? 2 : 1;
+    if (p.shared_inner == 0) return 0;
+    const int bytes = (p.fp8 ? 2 : 1) * ((p.T + kPassTokens - 1) / kPassTokens);
     return !DOWN ? bytes : min(max((p.shared_inner * bytes + p.F / 2) / p.F, 1), 64);
   }
-  __device__ int shared_column(int flat) const {
-    const int group = shared_cost() * 8;
-    return (flat - active * width() + group - 1) / group * 8;
-  }
-
+  __device__ int block_width() const { return DOWN ? min(kJoinColumns, p.D - block * kJoinColumns) : p.F; }
   __device__ bool next() {
     if (waiting > 0) {
       piece.begin += piece.n;
@@ -428,26 +427,36 @@ struct Stream {
     return true;
   }
   __device__ bool next_columns() {
-    if (at >= end) return false;
-    const int most = DOWN ? 256 : 128;
-    if (at < active * width()) {
-      piece.index = at / width();
-      piece.first = at - piece.index * width();
-      piece.count = min(min(most, width() - piece.first), end - at);
-      at += piece.count;
-      piece.fp8 = p.fp8;
-      piece.begin = l.begin[piece.index];
-      waiting = l.begin[piece.index + 1] - piece.begin;
-    } else {
-      piece.index = active;
-      piece.first = shared_column(at);
-      const int last = shared_column(end);
-      piece.count = min(most, last - piece.first);
-      if (piece.count <= 0) return false;
-      at = piece.first + piece.count < last ? active * width() + shared_cost() * (piece.first + piece.count) : end;
-      piece.fp8 = false;
-      piece.begin = 0;
-      waiting = p.T;
+    const int most = DOWN ? 256 : 128, cost = shared_cost();
+    for (;;) {
+      if (at >= end) return false;
+      const int size = kJoinColumns * (active + cost);  // of a whole block
+      block = DOWN ? at / size : 0;
+      const int width = block_width(), shared_width = DOWN ? width : p.shared_inner;
+      const int base = block * size, routed = base + active * width;
+      block_end = routed + cost * shared_width;
+      if (at < routed) {
+        piece.index = (at - base) / width;
+        const int column = at - base - piece.index * width;
+        piece.first = block * kJoinColumns + column;
+        piece.count = min(min(most, width - column), end - at);
+        at += piece.count;
+        piece.fp8 = p.fp8;
+        piece.begin = l.begin[piece.index];
+        waiting = l.begin[piece.index + 1] - piece.begin;
+      } else {
+        const int group = cost * 8, stop = min(end, block_end);
+        const int column = (at - routed + group - 1) / group * 8, last = (stop - routed + group - 1) / group * 8;
+        piece.index = active;
+        piece.first = block * kJoinColumns + column;
+        piece.count = min(most, last - column);
+        at = column + piece.count < last ? routed + cost * (column + piece.count) : stop;
+        if (piece.count <= 0) continue;
+        piece.fp8 = false;
+        piece.begin = 0;
+        waiting = p.T;
+      }
+      break;
     }
     const int tiles = DOWN ? (piece.count + 15) / 16 : (piece.count + 7) / 8;
     piece.rt_log = tiles <= 1 ? 0 : 32 - __clz(tiles - 1);
@@ -471,11 +480,10 @@ constexpr long long kPrefetchBytes = 256 << 10;
 __device__ __forceinline__ void prefetch_down(const DecodeParams& p, const Lists& l, int active) {
   Stream<true> now(p, l, active);
   const long long pitch = (long long)p.F * (p.fp8 ? 1 : 2);
-  int last = -1;
-  for (long long left = kPrefetchBytes; left > 0 && now.next() && now.piece.index < active;) {
-    if (now.piece.index == last && now.piece.begin > l.begin[last]) continue;  // another pass over the same rows
-    last = now.piece.index;
-    const uint8_t* from = p.w2 + ((long long)l.expert[last] * p.D + now.piece.first) * pitch;
+  for (long long left = kPrefetchBytes; left > 0 && now.next();) {
+    const int e = now.piece.index;
+    if (e == active || now.piece.begin > l.begin[e]) continue;  // (the shared expert; another pass over the same rows)
+    const uint8_t* from = p.w2 + ((long long)l.expert[e] * p.D + now.piece.first) * pitch;
     const long long bytes = min(left, now.piece.count * pitch);
     for (long long at = 0; at < bytes; at += 16384)
       asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(from + at), "r"((uint32_t)min(16384LL, bytes - at))
