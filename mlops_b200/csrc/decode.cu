@@ -47,7 +47,7 @@ constexpr int kTokenBytes = 256;      // a token's 128 columns beside an E4M3 bl
 constexpr int kTokenPitchBf16 = 192;  // its 64 beside a bf16 block: rows start in different banks
 constexpr int kStageScales = 2 * kStageSlabs;  // of the weights: each slab's first and other eight rows
 constexpr int kMaxStages = 8;
-constexpr int kJoinColumns = 256;
+constexpr int kBlockColumns = 256;    // of y that the down product takes together (Stream)
 constexpr int kPassTokens = 32;  // of one expert that a pass over its weights takes; rarely has an expert more
 
 __device__ __forceinline__ void copy16(void* dst, const void* src, bool read) {
@@ -61,37 +61,6 @@ __device__ __forceinline__ void copies_arrive(uint64_t* bar) {
 
 __device__ __forceinline__ void copy4(void* dst, const void* src) {
   asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(smem_u32(dst)), "l"(src) : "memory");
-}
-
-// mbar_wait for a whole warp whose poll sleeps up to 100 us at a time: what waits here waits for HBM, and polling took a third
-// of the SM's issue slots.
-__device__ __forceinline__ bool wait_stage(uint64_t* bar, uint32_t parity, volatile int* abort_flag, int* status,
-                                           int where) {
-  int ok = 1;
-  if ((threadIdx.x & 31) == 0) {
-    const long long start = clock64();
-    for (;;) {
-      uint32_t done;
-      asm volatile(
-          "{\n\t.reg .pred P;\n\t"
-          "mbarrier.try_wait.parity.shared::cta.b64 P, [%1], %2, 100000;\n\t"
-          "selp.u32 %0, 1, 0, P;\n\t}"
-          : "=r"(done)
-          : "r"(smem_u32(bar)), "r"(parity)
-          : "memory");
-      if (done) break;
-      const bool late = clock64() - start > B200_WAIT_LIMIT_CYCLES;
-      if (*abort_flag || late) {
-        if (late) {
-          *abort_flag = 1;
-          report_error(status, ERR_WAIT_TIMEOUT, where, (int)parity);
-        }
-        ok = 0;
-        break;
-      }
-    }
-  }
-  return __shfl_sync(0xffffffffu, ok, 0) != 0;
 }
 
 __device__ __forceinline__ void mma_f16(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
@@ -386,7 +355,7 @@ struct Piece {
   bool fp8;
 };
 
-// Their order: UP expert by expert, the shared one last; DOWN the same within each kJoinColumns columns (a block), .
+// Their order: UP expert by expert, the shared one last; DOWN the same within each kBlockColumns columns (a block), .
 template <bool DOWN>
 struct Stream {
   const DecodeParams& p;
@@ -412,7 +381,7 @@ struct Stream {
     const int bytes = (p.fp8 ? 2 : 1) * ((p.T + kPassTokens - 1) / kPassTokens);
     return !DOWN ? bytes : min(max((p.shared_inner * bytes + p.F / 2) / p.F, 1), 64);
   }
-  __device__ int block_width() const { return DOWN ? min(kJoinColumns, p.D - block * kJoinColumns) : p.F; }
+  __device__ int block_width() const { return DOWN ? min(kBlockColumns, p.D - block * kBlockColumns) : p.F; }
   __device__ bool next() {
     if (waiting > 0) {
       piece.begin += piece.n;
@@ -426,11 +395,14 @@ struct Stream {
     piece.steps = (piece.blocks + (1 << piece.ks_log) - 1) >> piece.ks_log;
     return true;
   }
+  // Of `left` columns those of a piece: half of `most`, twice the K blocks to a stage, where all of them would leave
+  // more than a quarter of the stages empty.
+  __device__ static int fill(int left, int most) { return left > most / 2 && left < most * 3 / 4 ? most / 2 : min(left, most); }
   __device__ bool next_columns() {
     const int most = DOWN ? 256 : 128, cost = shared_cost();
     for (;;) {
       if (at >= end) return false;
-      const int size = kJoinColumns * (active + cost);  // of a whole block
+      const int size = kBlockColumns * (active + cost);  // of a whole block
       block = DOWN ? at / size : 0;
       const int width = block_width(), shared_width = DOWN ? width : p.shared_inner;
       const int base = block * size, routed = base + active * width;
@@ -438,8 +410,8 @@ struct Stream {
       if (at < routed) {
         piece.index = (at - base) / width;
         const int column = at - base - piece.index * width;
-        piece.first = block * kJoinColumns + column;
-        piece.count = min(min(most, width - column), end - at);
+        piece.first = block * kBlockColumns + column;
+        piece.count = fill(min(width - column, end - at), most);
         at += piece.count;
         piece.fp8 = p.fp8;
         piece.begin = l.begin[piece.index];
@@ -448,8 +420,8 @@ struct Stream {
         const int group = cost * 8, stop = min(end, block_end);
         const int column = (at - routed + group - 1) / group * 8, last = (stop - routed + group - 1) / group * 8;
         piece.index = active;
-        piece.first = block * kJoinColumns + column;
-        piece.count = min(most, last - column);
+        piece.first = block * kBlockColumns + column;
+        piece.count = fill(last - column, most);
         at = column + piece.count < last ? routed + cost * (column + piece.count) : stop;
         if (piece.count <= 0) continue;
         piece.fp8 = false;
@@ -531,7 +503,7 @@ __device__ __forceinline__ void keep_full(const DecodeParams& p, const DecodeMap
       if ((stage & (kFillWarps - 1)) == turn) {
         const int block0 = step << piece.ks_log, here = min(ks_count, piece.blocks - block0);  // K blocks of this stage
         const int rows = here * piece.n;
-        if (stage >= count && !wait_stage(&bars.empty[slot], phase ^ 1, &bars.abort, p.status, 70)) {
+        if (stage >= count && !mbar_wait_warp(&bars.empty[slot], phase ^ 1, &bars.abort, p.status, 70)) {
           dead = true;
           break;
         }
@@ -742,7 +714,7 @@ stream_kernel(const DecodeParams p, const __grid_constant__ DecodeMaps maps, int
     const bool fp8 = piece.fp8;
     int block = ks;
     for (int step = piece.steps; step > 0; --step, block += ks_count) {
-      if (!dead) dead = !wait_stage(&bars.full[slot], phase, &bars.abort, p.status, 72);
+      if (!dead) dead = !mbar_wait_warp(&bars.full[slot], phase, &bars.abort, p.status, 72);
       if (block < blocks) {
         const uint32_t a = a_first + slot * kStageA, b = b_first + slot * p.b_rows * kTokenBytes;
         if (fp8)

@@ -91,7 +91,20 @@ route_topk_kernel(const float* __restrict__ logits, long long ld, int T, int E, 
         return best;
       };
       uint32_t my_group = 0;  // lane g holds the key of group g's score; 0: no such group, or taken
-      for (int g = 0; g < n_group; ++g) {
+      // groups of 32 experts are the registers themselves, and their maxima do not wait for one another (64 tokens
+      // of 256 experts in 8 groups: 7.2 us instead of 8.3)
+      if (gs == 32) {
+#pragma unroll
+        for (int j = 0; j < EPL; ++j) {
+          if (j < n_group) {
+            const uint32_t top = __reduce_max_sync(0xffffffffu, keys[j]);
+            const int winner = __ffs(__ballot_sync(0xffffffffu, keys[j] == top)) - 1;  // the lowest id that holds it
+            const uint32_t second = __reduce_max_sync(0xffffffffu, lane == winner ? 0u : keys[j]);
+            if (lane == j) my_group = order_key(key_value(top) + key_value(second));
+          }
+        }
+      }
+      for (int g = gs == 32 ? n_group : 0; g < n_group; ++g) {
         const int lo = g * gs, hi = lo + gs;
         int id;
         const uint32_t mine = best_in(lo, hi, -1, id);

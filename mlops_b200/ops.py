@@ -1232,5 +1232,5 @@ def moe_decode(x, residual, router, w13, w2, *, top_k, mode, bias=None, n_group=
         w13.data_ptr(), _ptr(s13), w2.data_ptr(), _ptr(s2), _ptr(shared13), _ptr(shared2), weights.data_ptr(),
         ids.data_ptr(), output.data_ptr(), workspace.data_ptr(), status_block(device).data_ptr())
     check(lib.b200moe_decode(ctypes.byref(args), _stream()), "moe_decode")
-    _count(4)
+    _count(5 if s13 is None else 6)
     return output, weights, ids
