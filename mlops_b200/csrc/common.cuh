@@ -478,18 +478,20 @@ __device__ __forceinline__ Float2 mad2(Float2 a, Float2 b, Float2 c) {
 // reciprocal; the true quotient lies within 2^-22 (relative) of that product, and the cast is
 // monotonic, so when both ends of the interval [q(1-2^-21), q(1+2^-21)] cast to the same
 // byte that byte is the exact answer.  Otherwise (a value within an ulp of an E4M3 rounding
-// boundary, about one lane in ten thousand) the eight values take the exact division.
+// boundary, about one lane in ten thousand) the eight values take the exact division.  (The ends are products and
+// not fma(q, +-2^-21, q), which has the same bits but makes the two ends of a -0 differ in sign: where gradients hold
+// zeros nearly every warp then divided, 427 us instead of 309 for 65536 rows of F = 2048.)
 __device__ __forceinline__ uint2 quantize8(const float (&v)[8], float scale) {
   const Float2 inv = splat2(__frcp_rn(scale));
-  const Float2 up = splat2(4.76837158203125e-7f), down = splat2(-4.76837158203125e-7f);  // 2^-21
+  const Float2 up = splat2(1.000000476837158203125f), down = splat2(0.999999523162841796875f);  // 1 +- 2^-21
   uint32_t w[2] = {0, 0};
   bool exact = true;
 #pragma unroll
   for (int i = 0; i < 8; i += 2) {
     const Float2 q = mul2(pack2(v[i], v[i + 1]), inv);
     float2 above, below;
-    unpack2(mad2(q, up, q), above.x, above.y);
-    unpack2(mad2(q, down, q), below.x, below.y);
+    unpack2(mul2(q, up), above.x, above.y);
+    unpack2(mul2(q, down), below.x, below.y);
     const uint32_t hi = __nv_cvt_float2_to_fp8x2(above, __NV_SATFINITE, __NV_E4M3);
     const uint32_t lo = __nv_cvt_float2_to_fp8x2(below, __NV_SATFINITE, __NV_E4M3);
     exact = exact && (hi == lo);

@@ -53,13 +53,19 @@ __device__ __forceinline__ uint32_t largest_bits(const uint4& raw) {
   return max(m & 0xffffu, m >> 16);
 }
 
+// Both quotients of both halves by one division a lane: of four neighbouring lanes 0 and 1 form 127 / a of the gate and
+// the up block, 2 and 3 a / 127, and keep them (`scale` is right in those lanes alone).  Four divisions a lane took
+// a fifth of the kernel's instructions.
 struct CodeFactors {
-  float scale, inverse;
+  float inverse_gate, inverse_up, scale;
 };
-__device__ __forceinline__ CodeFactors code_factors(uint32_t bits) {
+__device__ __forceinline__ CodeFactors code_factors(uint32_t gate_bits, uint32_t up_bits, int lane) {
+  const uint32_t bits = (lane & 1) ? up_bits : gate_bits;
   const float a = fmaxf(__uint_as_float(bits << 16), kCodeFloor);
-  if (bits >= 0x7f80u) return {__int_as_float(0x7fc00000), 0.0f};
-  return {__fdiv_rn(a, 127.0f), __fdiv_rn(127.0f, a)};
+  const bool scales = (lane & 2) != 0;
+  float quotient = __fdiv_rn(scales ? a : 127.0f, scales ? 127.0f : a);
+  if (bits >= 0x7f80u) quotient = scales ? __int_as_float(0x7fc00000) : 0.0f;
+  return {__shfl_sync(0xffffffffu, quotient, lane & 28), __shfl_sync(0xffffffffu, quotient, (lane & 28) + 1), quotient};
 }
 
 __device__ __forceinline__ uint2 encode8(const float (&v)[8], float inverse) {
@@ -263,17 +269,15 @@ swiglu_quant_kernel(const __nv_bfloat16* __restrict__ h13, long long ldh, long l
       uint32_t m = largest_bits(rg) | (largest_bits(ru) << 16);
 #pragma unroll
       for (int o = 8; o > 0; o >>= 1) m = max_u16x2(m, __shfl_xor_sync(0xffffffffu, m, o));
-      const CodeFactors fg = code_factors(m & 0xffffu), fu = code_factors(m >> 16);
+      const CodeFactors f = code_factors(m & 0xffffu, m >> 16, lane);
       if (c < F) {
         int8_t* code = saved.codes + r * saved.ld + c;
-        *reinterpret_cast<uint2*>(code) = encode8(g, fg.inverse);
-        *reinterpret_cast<uint2*>(code + F) = encode8(u, fu.inverse);
-        if ((lane & 15) == 0) {
-          float* scale = saved.scales + r * saved.s_row + (long long)(c >> 7) * saved.s_block;
-          scale[0] = fg.scale;
-          scale[(long long)((F + 127) >> 7) * saved.s_block] = fu.scale;
-        }
+        *reinterpret_cast<uint2*>(code) = encode8(g, f.inverse_gate);
+        *reinterpret_cast<uint2*>(code + F) = encode8(u, f.inverse_up);
       }
+      const int block = (c - (lane & 15) * 8) >> 7;  // of this half of the warp; its lanes 2 and 3 have the scales
+      if ((lane & 14) == 2 && block * 128 < F)
+        saved.scales[r * saved.s_row + (block + ((lane & 1) ? (F + 127) >> 7 : 0)) * saved.s_block] = f.scale;
     }
     fetch(c + 256);
     if constexpr (LIMITED) {

@@ -130,7 +130,7 @@ def _ptr(t) -> int | None:
 def status_block(device) -> torch.Tensor:
     """The per-device int32[4] block the kernels report bounded-wait and validation
     failures into. Created (zeroed) on first use."""
-    index = torch.device(device).index
+    index = device.index if isinstance(device, torch.device) else torch.device(device).index
     if index is None:
         index = torch.cuda.current_device()
     block = _STATUS.get(index)
@@ -282,7 +282,9 @@ def sort_assignments_static(route_ids, experts, order, offsets, slots, counts):
 def _scale_buffer(rows, blocks, device):
     """Scales are stored block-major ([blocks, rows]) so that the GEMM epilogue's 32
     lanes read 32 consecutive floats; the returned view is [rows, blocks]."""
-    return torch.empty((blocks, max(rows, 1)), dtype=torch.float32, device=device)[:, :rows].t()
+    if rows:
+        return torch.empty((blocks, rows), dtype=torch.float32, device=device).t()
+    return torch.empty((blocks, 1), dtype=torch.float32, device=device)[:, :0].t()
 
 
 @_on_tensor_device
@@ -423,11 +425,13 @@ def _saved_blocks(width):
 
 def _check_saved(codes, scales):
     """`(rows, width)` of kept rows; their layout is what `swiglu_save8` writes, with any row pitch."""
-    if (codes.dtype != torch.int8 or codes.dim() != 2 or codes.shape[1] % 16 or codes.shape[1] == 0
-            or (codes.shape[0] > 0 and codes.stride(1) != 1)):
+    if codes.dtype != torch.int8 or codes.dim() != 2:
         raise NativeError("kept rows are int8 [rows, 2F] with unit inner stride, F a multiple of 8")
-    rows, width = codes.shape[0], codes.shape[1] // 2
-    if scales.dtype != torch.float32 or tuple(scales.shape) != (rows, _saved_blocks(width)):
+    rows, two_f = codes.shape
+    if two_f % 16 or two_f == 0 or (rows > 0 and codes.stride(1) != 1):
+        raise NativeError("kept rows are int8 [rows, 2F] with unit inner stride, F a multiple of 8")
+    width = two_f // 2
+    if scales.dtype != torch.float32 or scales.shape != (rows, _saved_blocks(width)):
         raise NativeError(f"their scales are fp32 [rows, 2 ceil(F / 128)] = [{rows}, {_saved_blocks(width)}]")
     return rows, width
 
@@ -499,13 +503,13 @@ def dswiglu_saved8(saved, r, route_weights, order, *, limit=None, quantized=True
 def _dswiglu_saved8(codes, code_scales, r, route_weights, order, limit, quantized, rounded, scaled_activation):
     device = _need_cuda(codes, code_scales, r, route_weights, order)
     rows, width = _check_saved(codes, code_scales)
-    if r.dtype != torch.bfloat16 or tuple(r.shape) != (rows, width) or (rows > 0 and r.stride(1) != 1):
+    if r.dtype != torch.bfloat16 or r.shape != (rows, width) or (rows > 0 and r.stride(1) != 1):
         raise NativeError(f"r must be bf16 [{rows}, {width}] with unit inner stride")
     if quantized and width % 128:
         raise NativeError("the E4M3 gradient needs F to be a multiple of 128")
     if order.dtype != torch.int32 or not order.is_contiguous() or order.numel() != rows:
         raise NativeError("order must be contiguous int32 with one entry per row")
-    weights = route_weights.reshape(-1)
+    weights = route_weights if route_weights.dim() == 1 and route_weights.is_contiguous() else route_weights.reshape(-1)
     if weights.dtype != torch.float32 or (rows > 0 and weights.numel() == 0):
         raise NativeError("route_weights must be fp32 and not empty")
     two_f = 2 * width
