@@ -8,11 +8,12 @@
 //   out[t] = residual[t] + sum_k w[t,k] y[t,k] (+ the shared expert's)   join_kernel
 //
 // Bound: HBM.  The weights of the experts that got a token are read once, 3 D F bytes each in E4M3, for one
-// or a few multiplications a byte; everything else is small.  So the two products are one stream of weight
-// rows through shared memory (boxes of 128 bytes of K, several stages of 32 KB in flight per SM), and the rows of all experts
-// with tokens, one after the other, are cut evenly over the CTAs in groups of eight: with whole tiles of 64 columns
-// eight experts of F = 768 would leave 52 of 148 SMs idle.  Cutting the down product's output columns instead, which
-// needs no y, left a CTA 14 to 24 rows of each expert: the tokens' columns then weigh as much as the weights'.
+// or a few multiplications a byte; everything else is small.  So each product is one stream of weight rows
+// through shared memory (boxes of 128 bytes of K, several stages of 32 KB in flight per SM), and the rows of all
+// experts with tokens, one after the other, are cut evenly over the CTAs in groups of eight: with whole tiles of 64
+// columns eight experts of F = 768 would leave 52 of 148 SMs idle.  Cutting the down product's output columns
+// instead, which needs no y, left a CTA 14 to 24 rows of each expert: the tokens' columns then weigh as much as
+// the weights'.
 //
 // The weights are the A operand of mma.sync.m16n8k16 (16 weight rows), the tokens the B operand (8 to a tile).
 // Against bf16 weights the tokens are bf16.  E4M3 weights are widened to f16, one instruction for two values, and a
@@ -355,7 +356,7 @@ struct Piece {
   bool fp8;
 };
 
-// Their order: UP expert by expert, the shared one last; DOWN the same within each kBlockColumns columns (a block), .
+// Their order: UP expert by expert, the shared one last; DOWN the same within each kBlockColumns columns of y (a block).
 template <bool DOWN>
 struct Stream {
   const DecodeParams& p;

@@ -672,6 +672,35 @@ def apply(h2, residual, router_weight, w13_experts, w2_experts, *, top_k, routin
     return outputs[:4]
 
 
+def decode(h2, residual, router_weight, w13_experts, w2_experts, *, top_k, routing_mode, router_bias=None, n_group=1,
+           topk_group=1, routed_scaling=1.0, shared_w13=None, shared_w2=None, shared_gate_weight=None,
+           shared_mode="add", swiglu_limit=None):
+    """`apply`'s output for the 1 to 64 tokens of a serving loop, without statistics and without a gradient:
+    `layer.forward_decode` on the same arguments, weight containers included. Activations stay bf16 on
+    block-FP8 experts as well, so the two differ by the E4M3 rounding of `apply`'s activations. Refuses, with
+    the reason, what it does not take: more tokens, a call that autograd would have to follow."""
+    reason = refusal(h2, residual, router_weight, w13_experts, w2_experts, top_k=top_k, routing_mode=routing_mode,
+                     n_group=n_group, topk_group=topk_group, shared_w13=shared_w13, shared_w2=shared_w2)
+    if reason is None and h2.numel() > kernels.DECODE_TOKENS * h2.shape[-1]:
+        reason = f"decode takes at most {kernels.DECODE_TOKENS} tokens: apply takes more"
+    if reason is None and torch.is_grad_enabled() and any(
+            t is not None and t.requires_grad for t in (h2, residual, router_weight, w13_experts, w2_experts,
+                                                       shared_w13, shared_w2, shared_gate_weight)):
+        reason = "decode has no gradient: call it under torch.no_grad(), or use apply"
+    if reason is not None:
+        raise ValueError(reason)
+    shared = None
+    if shared_w13 is not None:
+        if shared_mode == "add" and shared_w13.is_contiguous() and shared_w2.is_contiguous():
+            shared = (shared_w13, shared_w2)
+        else:  # gated, or of strides the kernels do not read
+            residual = residual + shared_expert(h2, shared_w13, shared_w2, shared_gate_weight, shared_mode, swiglu_limit)
+    return layer.forward_decode(
+        h2, residual, router_weight, _operands(w13_experts), _operands(w2_experts), top_k=int(top_k),
+        routing_mode=str(routing_mode), router_bias=router_bias, n_group=int(n_group), topk_group=int(topk_group),
+        routed_scaling=float(routed_scaling), swiglu_limit=swiglu_limit, shared=shared)[0]
+
+
 def forward(h2, residual, router_weight, w13_experts, w2_experts, *, top_k, routing_mode, router_bias=None,
             n_group=1, topk_group=1, routed_scaling=1.0, lengths=None, weight_precision="float32",
             swiglu_implementation=None, swiglu_limit=None):

@@ -73,3 +73,12 @@ def test_the_wrapper_refuses_what_it_does_not_take():
         with pytest.raises(NativeError):
             call(first, second)
     assert ops.DECODE_TOKENS == 64
+
+
+def test_the_provider_refuses_with_the_reason():
+    from mlops_b200 import provider
+
+    x = torch.zeros(4, 256, dtype=torch.bfloat16)
+    w13, w2 = torch.zeros(8, 256, 256, dtype=torch.bfloat16), torch.zeros(8, 256, 128, dtype=torch.bfloat16)
+    with pytest.raises(ValueError, match="CUDA"):
+        provider.decode(x, x, torch.zeros(8, 256), w13, w2, top_k=2, routing_mode="softmax_then_topk")
