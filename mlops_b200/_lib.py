@@ -7,6 +7,7 @@ from __future__ import annotations
 
 import ctypes
 import os
+import struct
 from ctypes import c_float, c_int, c_int32, c_longlong, c_void_p
 from pathlib import Path
 
@@ -61,6 +62,12 @@ class DecodeArgs(ctypes.Structure):
         "shared_inner")] + [("routed_scaling", F), ("limit", F)] + [(n, P) for n in (
             "x", "residual", "router", "bias", "w13", "w13_scale", "w2", "w2_scale", "shared_w13", "shared_w2",
             "route_weights", "ids", "output", "workspace", "status")]
+
+
+# The same as bytes, which the entry point takes for a pointer: a third of the Structure's time on the host (1.3 against
+# 4 us of a call that takes 33).
+pack_decode_args = struct.Struct("@q10i2f15P").pack
+assert struct.calcsize("@q10i2f15P") == ctypes.sizeof(DecodeArgs)
 
 
 # name -> (restype, argtypes); one entry per declaration in include/b200moe.h

@@ -100,20 +100,19 @@ __device__ __forceinline__ float scale_row(const __nv_bfloat16* __restrict__ fro
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   uint32_t m = 0;
 #pragma unroll 4
-  for (int i = threadIdx.x; i < width / 4; i += kDecodeThreads) {
+  for (int i = threadIdx.x; i < width / 4; i += blockDim.x) {
     const uint2 raw = in[i];
     m = __vmaxu2(m, __vmaxu2(raw.x & 0x7fff7fffu, raw.y & 0x7fff7fffu));
   }
   m = __reduce_max_sync(0xffffffffu, max(m & 0xffffu, m >> 16));
   if (lane == 0) largest[warp] = m;
   __syncthreads();
-#pragma unroll
-  for (int w = 0; w < kDecodeWarps; ++w) m = max(m, largest[w]);
+  m = __reduce_max_sync(0xffffffffu, lane < blockDim.x / 32 ? largest[lane] : 0u);
   // exponent of the largest, kept where both powers of two are normal numbers
   const int e = min(max((int)(m >> 7), 27), 254);
   const float inverse = __int_as_float((268 - e) << 23);  // largest / s in [2^14, 2^15)
 #pragma unroll 4
-  for (int i = threadIdx.x; i < width / 4; i += kDecodeThreads) {
+  for (int i = threadIdx.x; i < width / 4; i += blockDim.x) {
     const uint2 raw = in[i];
     const __nv_bfloat162* pairs = reinterpret_cast<const __nv_bfloat162*>(&raw);
     const float2 a = __bfloat1622float2(pairs[0]), b = __bfloat1622float2(pairs[1]);
@@ -250,62 +249,81 @@ struct DecodeParams {
   int* status;
 };
 
-// Weight rows as [experts * rows, K], read in boxes of `tall` (UP: 128, DOWN: 256) or 8 rows x 128 bytes.
-struct DecodeMaps {
-  CUtensorMap tall, flat, shared_tall, shared_flat;
+// Weight rows as [experts * rows, K], read in boxes of 128 bytes of K by 8, 32 or all rows of a full piece (UP: 128, DOWN:
+// 256).  (A box takes the copy unit 50 cycles, 8 rows of it as much as 32: by eights alone the down product of F = 14336
+// ran at 4.8 TB/s.)
+struct WeightMaps {
+  CUtensorMap tall, middle, flat;
 };
+struct DecodeMaps {
+  WeightMaps routed, shared;
+};
+// Weights are read once: they go through L2 as the first to leave it, so that the kernels' own instructions, the tokens and
+// the lists stay (a call that streamed 448 MB fetched its instructions from HBM again).
+__device__ __forceinline__ uint64_t read_once() {
+  uint64_t policy;
+  asm("createpolicy.fractional.L2::evict_first.b64 %0, 1.0;" : "=l"(policy));
+  return policy;
+}
+__device__ __forceinline__ void load_box(void* to, const CUtensorMap* map, uint64_t* full, int x, int y, uint64_t policy) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.shared::cta.global.mbarrier::complete_tx::bytes.L2::cache_hint [%0], [%1, {%3, %4}], [%2], %5;" ::"r"(
+          smem_u32(to)),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(smem_u32(full)), "r"(x), "r"(y), "l"(policy)
+      : "memory");
+}
+__device__ __forceinline__ void load_rows(uint8_t* to, const WeightMaps& maps, uint64_t* full, int x, int y, int count,
+                                          uint64_t policy) {
+  int row = 0;
+  for (; row + 32 <= count; row += 32) load_box(to + row * 128, &maps.middle, full, x, y + row, policy);
+  for (; row < count; row += 8) load_box(to + row * 128, &maps.flat, full, x, y + row, policy);
+}
 
 // Where things are in shared memory behind the stages.
 struct Lists {
-  int* begin;          // [experts with tokens + 1] first row of each
-  uint16_t* expert;    // [experts with tokens]
-  uint8_t* tokens;     // [T * K]
-  float* scale;        // [T * K] UP, E4M3: the power of two of each row's token
-  int* scratch;        // [E + 64]
-  uint16_t* rank;      // [T * K]
+  int* begin;         // [experts with tokens + 1] first row of each
+  float* scale;       // [T * K] UP, E4M3: the power of two of each row's token
+  uint32_t* mask;     // [E][2] the tokens of each expert
+  int* totals;        // [warps]
+  uint16_t* expert;   // [experts with tokens]
+  uint16_t* first;    // [E] first row of each
+  uint8_t* tokens;    // [T * K]
   __host__ __device__ static int bytes(int T, int E, int K) {
     const int R = T * K, most = E < R ? E : R;
-    return 4 * (most + 1) + 4 * R + 4 * (E + 64) + 2 * (most + R) + R + 64;
+    return 4 * (most + 1) + 4 * R + 8 * E + 4 * (kStreamThreads / 32) + 2 * (most + E) + R;
   }
   __device__ void place(uint8_t* base, int T, int E, int K) {
     const int R = T * K, most = E < R ? E : R;
     begin = reinterpret_cast<int*>(base);
     scale = reinterpret_cast<float*>(begin + most + 1);
-    scratch = reinterpret_cast<int*>(scale + R);
-    expert = reinterpret_cast<uint16_t*>(scratch + E + 64);
-    rank = expert + most;
-    tokens = reinterpret_cast<uint8_t*>(rank + R);
+    mask = reinterpret_cast<uint32_t*>(scale + R);
+    totals = reinterpret_cast<int*>(mask + 2 * E);
+    expert = reinterpret_cast<uint16_t*>(totals + kStreamThreads / 32);
+    first = expert + most;
+    tokens = reinterpret_cast<uint8_t*>(first + E);
   }
 };
 
-// Rows by expert, in token order inside one; returns the number of experts with tokens.
+// Rows by expert, in token order inside one; returns the number of experts with tokens.  A token has an expert at most
+// once, so an expert's tokens are a mask of 64 bits and a row's place in them a count of bits: nothing is serial.
+// (One warp that ranked 32 assignments at a time took 5 us longer for 48 tokens of 8.)
 __device__ __forceinline__ int build_lists(const Lists& l, const int* __restrict__ ids, int T, int E, int K,
                                            int* __restrict__ row_of, const float* __restrict__ token_scale) {
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, R = T * K;
-  int* count = l.scratch;           // per expert: rows, then first row
-  int* totals = l.scratch + E;      // per warp
-  for (int e = tid; e < E; e += kStreamThreads) count[e] = 0;
+  for (int e = tid; e < 2 * E; e += kStreamThreads) l.mask[e] = 0;
   __syncthreads();
-  if (warp == 0) {
-    for (int base = 0; base < R; base += 32) {
-      const int i = base + lane;
-      const bool in = i < R;
-      const int e = in ? ids[i] : -1 - lane;
-      const unsigned same = __match_any_sync(0xffffffffu, e);
-      const int before = __popc(same & ((1u << lane) - 1));
-      if (in) l.rank[i] = (uint16_t)(count[e] + before);
-      __syncwarp();
-      if (in && before == 0) count[e] += __popc(same);
-      __syncwarp();
-    }
+  for (int i = tid; i < R; i += kStreamThreads) {
+    const int token = i / K;
+    atomicOr(l.mask + 2 * ids[i] + (token >> 5), 1u << (token & 31));
   }
   __syncthreads();
   // exclusive sums over the experts of (rows, experts with rows), packed in one word
   const int per = (E + kStreamThreads - 1) / kStreamThreads;
+  const auto rows = [&](int e) { return e < E ? __popc(l.mask[2 * e]) + __popc(l.mask[2 * e + 1]) : 0; };
   int mine = 0;
   for (int j = 0; j < per; ++j) {
-    const int e = tid * per + j;
-    if (e < E && count[e]) mine += count[e] | (1 << 16);
+    const int n = rows(tid * per + j);
+    mine += n ? n | (1 << 16) : 0;
   }
   int incl = mine;
 #pragma unroll
@@ -313,19 +331,20 @@ __device__ __forceinline__ int build_lists(const Lists& l, const int* __restrict
     const int v = __shfl_up_sync(0xffffffffu, incl, o);
     if (lane >= o) incl += v;
   }
-  if (lane == 31) totals[warp] = incl;
+  if (lane == 31) l.totals[warp] = incl;
   __syncthreads();
-  int at = incl - mine;
-  for (int w = 0; w < warp; ++w) at += totals[w];
-  int active = 0;
-  for (int w = 0; w < kStreamThreads / 32; ++w) active += totals[w];
+  int at = incl - mine, active = 0;
+#pragma unroll
+  for (int w = 0; w < kStreamThreads / 32; ++w) {
+    const int n = l.totals[w];
+    if (w < warp) at += n;
+    active += n;
+  }
   active >>= 16;
   for (int j = 0; j < per; ++j) {
-    const int e = tid * per + j;
-    if (e >= E) break;
-    const int n = count[e];
-    count[e] = at & 0xffff;
+    const int e = tid * per + j, n = rows(e);
     if (n) {
+      l.first[e] = (uint16_t)at;
       l.expert[at >> 16] = (uint16_t)e;
       l.begin[at >> 16] = at & 0xffff;
       at += n | (1 << 16);
@@ -334,9 +353,10 @@ __device__ __forceinline__ int build_lists(const Lists& l, const int* __restrict
   if (tid == 0) l.begin[active] = R;
   __syncthreads();
   for (int i = tid; i < R; i += kStreamThreads) {
-    const int at_row = count[ids[i]] + l.rank[i];
+    const int token = i / K, e = ids[i];
+    const uint32_t low = l.mask[2 * e], high = l.mask[2 * e + 1], below = (1u << (token & 31)) - 1;
+    const int at_row = l.first[e] + (token < 32 ? __popc(low & below) : __popc(low) + __popc(high & below));
     if (row_of != nullptr) row_of[i] = at_row;
-    const int token = i / K;
     l.tokens[at_row] = (uint8_t)token;
     if (token_scale != nullptr) l.scale[at_row] = token_scale[token];
   }
@@ -476,14 +496,14 @@ __device__ __forceinline__ void keep_full(const DecodeParams& p, const DecodeMap
                                           int count, Barriers& bars) {
   const int lane = threadIdx.x & 31, turn = (threadIdx.x >> 5) - kMultiplyWarps;
   Stream<DOWN> now(p, l, active);
+  const uint64_t policy = read_once();
   int slot = 0, stage = 0;
   uint32_t phase = 0;
   bool dead = false;
   while (!dead && now.next()) {
     const Piece& piece = now.piece;
     const bool shared = piece.index == active;
-    const CUtensorMap* tall = shared ? &maps.shared_tall : &maps.tall;
-    const CUtensorMap* flat = shared ? &maps.shared_flat : &maps.flat;
+    const WeightMaps& weights = shared ? maps.shared : maps.routed;
     const int inner = now.inner(), ks_count = 1 << piece.ks_log;
     const int columns = piece.fp8 ? 128 : 64;  // of a K block
     const int up = shared ? p.shared_inner : p.F;
@@ -515,20 +535,12 @@ __device__ __forceinline__ void keep_full(const DecodeParams& p, const DecodeMap
           mbar_arrive_expect_tx(full, here * piece.count * (DOWN ? 128 : 256));
           for (int ks = 0; ks < here; ++ks, to += block_bytes) {
             const int x = (block0 + ks) * columns;
-            if (DOWN) {
-              if (piece.count == 256) {
-                tma_load_2d(to, tall, full, x, y);
-              } else {
-                for (int row = 0; row < piece.count; row += 8) tma_load_2d(to + row * 128, flat, full, x, y + row);
-              }
-            } else if (piece.count == 128) {
-              tma_load_2d(to, tall, full, x, y);
-              tma_load_2d(to + 16384, tall, full, x, y + up);
+            if (piece.count == (DOWN ? 256 : 128)) {
+              load_box(to, &weights.tall, full, x, y, policy);
+              if (!DOWN) load_box(to + 16384, &weights.tall, full, x, y + up, policy);
             } else {
-              for (int row = 0; row < piece.count; row += 8) {
-                tma_load_2d(to + row * 128, flat, full, x, y + row);
-                tma_load_2d(to + block_bytes / 2 + row * 128, flat, full, x, y + up + row);
-              }
+              load_rows(to, weights, full, x, y, piece.count, policy);
+              if (!DOWN) load_rows(to + block_bytes / 2, weights, full, x, y + up, piece.count, policy);
             }
           }
         }
@@ -669,8 +681,9 @@ stream_kernel(const DecodeParams p, const __grid_constant__ DecodeMaps maps, int
     }
     bars.abort = 0;
     fence_mbar_init();
-    tma_prefetch_desc(&maps.tall);
-    tma_prefetch_desc(&maps.flat);
+    tma_prefetch_desc(&maps.routed.tall);
+    tma_prefetch_desc(&maps.routed.middle);
+    tma_prefetch_desc(&maps.routed.flat);
   }
   __syncthreads();
   // UP starts from the routing; when its blocks have seen that finished they let the next kernels start, so that
@@ -773,10 +786,11 @@ stream_kernel(const DecodeParams p, const __grid_constant__ DecodeMaps maps, int
   }
 }
 
-// act [rows, F] for the E4M3 down product, a block to a row.
-__global__ void __launch_bounds__(kDecodeThreads)
+// act [rows, F] for the E4M3 down product, a block to a row.  Latency: 1024 threads where the row has more than four
+// loads for each of 256 (34 rows of 14336: 10 us with 256).
+__global__ void __launch_bounds__(1024)
 scale_act_kernel(const __nv_bfloat16* __restrict__ act, int F, __half* __restrict__ act16, float* __restrict__ act16_scale) {
-  __shared__ uint32_t largest[kDecodeWarps];
+  __shared__ uint32_t largest[32];
   const long long at = (long long)blockIdx.x * F;
   dependency_release();
   dependency_wait();
@@ -795,12 +809,25 @@ join_kernel(const DecodeParams p) {
   float v[4];
 #pragma unroll
   for (int i = 0; i < 4; ++i) v[i] = __bfloat162float(p.residual[at + i]);
-  for (int k = 0; k < p.K; ++k) {
-    const int row = p.row_of[t * p.K + k];
-    float w = p.route_weights[t * p.K + k];
-    if (p.fp8) w *= p.act16_scale[row];  // (a power of two)
-    const float4 y = *reinterpret_cast<const float4*>(p.y + (long long)row * p.D + c);
-    v[0] = fmaf(w, y.x, v[0]), v[1] = fmaf(w, y.y, v[1]), v[2] = fmaf(w, y.z, v[2]), v[3] = fmaf(w, y.w, v[3]);
+  for (int k0 = 0; k0 < p.K; k0 += 8) {  // eight rows asked for at once
+    float w[8];
+    float4 y[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      if (k0 + i < p.K) {
+        const int row = p.row_of[t * p.K + k0 + i];
+        w[i] = p.route_weights[t * p.K + k0 + i];
+        if (p.fp8) w[i] *= p.act16_scale[row];  // (a power of two)
+        y[i] = *reinterpret_cast<const float4*>(p.y + (long long)row * p.D + c);
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      if (k0 + i < p.K) {
+        v[0] = fmaf(w[i], y[i].x, v[0]), v[1] = fmaf(w[i], y[i].y, v[1]);
+        v[2] = fmaf(w[i], y[i].z, v[2]), v[3] = fmaf(w[i], y[i].w, v[3]);
+      }
+    }
   }
   if (p.shared_inner > 0) {
     const float4 y = *reinterpret_cast<const float4*>(p.y + (long long)(p.T * p.K + t) * p.D + c);
@@ -894,7 +921,8 @@ static int launch_streams(const DecodeParams& p, const DecodeMaps& up, const Dec
   int code = launch_stream<false, MOST>(p, up, s);
   if (code != B200MOE_OK) return code;
   if (p.fp8) {
-    code = launch_dependent(scale_act_kernel, p.T * p.K, kDecodeThreads, 0, s, true, p.act, p.F, p.act16, p.act16_scale);
+    const int threads = p.F > 16 * kDecodeThreads ? 1024 : kDecodeThreads;
+    code = launch_dependent(scale_act_kernel, p.T * p.K, threads, 0, s, true, p.act, p.F, p.act16, p.act16_scale);
     if (code != B200MOE_OK) return code;
   }
   code = launch_stream<true, MOST>(p, down, s);
@@ -937,18 +965,16 @@ extern "C" int b200moe_decode(const b200moe_decode_args* a, void* stream) {
   DecodeMaps up, down;
   const long long E = a->experts, D = a->width, F = a->inner, Fs = a->shared_inner;
   int code = B200MOE_OK;
-  const auto encode = [&](CUtensorMap& map, const void* weights, bool e4m3, long long rows, long long k, int height) {
-    if (code == B200MOE_OK) code = encode_weights(&map, weights, e4m3, rows, k, height);
+  const auto encode = [&](WeightMaps& maps, const void* weights, bool e4m3, long long rows, long long k, int tall) {
+    if (code == B200MOE_OK) code = encode_weights(&maps.tall, weights, e4m3, rows, k, tall);
+    if (code == B200MOE_OK) code = encode_weights(&maps.middle, weights, e4m3, rows, k, 32);
+    if (code == B200MOE_OK) code = encode_weights(&maps.flat, weights, e4m3, rows, k, 8);
   };
-  encode(up.tall, a->w13, fp8, 2 * E * F, D, 128);
-  encode(up.flat, a->w13, fp8, 2 * E * F, D, 8);
-  encode(down.tall, a->w2, fp8, E * D, F, 256);
-  encode(down.flat, a->w2, fp8, E * D, F, 8);
+  encode(up.routed, a->w13, fp8, 2 * E * F, D, 128);
+  encode(down.routed, a->w2, fp8, E * D, F, 256);
   if (Fs > 0) {
-    encode(up.shared_tall, a->shared_w13, false, 2 * Fs, D, 128);
-    encode(up.shared_flat, a->shared_w13, false, 2 * Fs, D, 8);
-    encode(down.shared_tall, a->shared_w2, false, D, Fs, 256);
-    encode(down.shared_flat, a->shared_w2, false, D, Fs, 8);
+    encode(up.shared, a->shared_w13, false, 2 * Fs, D, 128);
+    encode(down.shared, a->shared_w2, false, D, Fs, 256);
   }
   if (code != B200MOE_OK) return code;
   const DecodeWorkspace w(a->tokens, a->width, a->experts, a->top_k, a->inner, a->shared_inner);

@@ -16,7 +16,7 @@ import os
 
 import torch
 
-from ._lib import BackwardArgs, DecodeArgs, ForwardArgs, NativeError, check, lib
+from ._lib import BackwardArgs, ForwardArgs, NativeError, check, lib, pack_decode_args
 
 ROUTING_MODES = {"topk_then_softmax": 0, "softmax_then_topk": 1, "sigmoid_noaux_tc": 2}
 FP8 = torch.float8_e4m3fn
@@ -1189,6 +1189,11 @@ def _decode_weights(w13, w2):
     return w13, scales[0], w2, scales[1]
 
 
+@functools.lru_cache(maxsize=256)
+def _decode_workspace(*sizes):
+    return lib.b200moe_decode_workspace_bytes(*sizes)
+
+
 @_on_tensor_device
 def moe_decode(x, residual, router, w13, w2, *, top_k, mode, bias=None, n_group=1, topk_group=1, routed_scaling=1.0,
                limit=None, shared=None):
@@ -1227,14 +1232,15 @@ def moe_decode(x, residual, router, w13, w2, *, top_k, mode, bias=None, n_group=
     ids = torch.empty((tokens, top_k), dtype=torch.int32, device=device)
     if tokens == 0:
         return output, weights, ids
-    workspace = torch.empty(lib.b200moe_decode_workspace_bytes(tokens, width, inner, experts, top_k, shared_inner),
-                            dtype=torch.uint8, device=device)
-    args = DecodeArgs(
-        tokens, width, inner, experts, top_k, ROUTING_MODES[mode], int(n_group), int(topk_group),
-        0 if limit is None else 1, 1 if router.dtype == torch.float32 else 0, shared_inner, float(routed_scaling),
-        0.0 if limit is None else float(limit), x.data_ptr(), residual.data_ptr(), router.data_ptr(), _ptr(bias),
-        w13.data_ptr(), _ptr(s13), w2.data_ptr(), _ptr(s2), _ptr(shared13), _ptr(shared2), weights.data_ptr(),
+    workspace = torch.empty(_decode_workspace(tokens, width, inner, experts, top_k, shared_inner), dtype=torch.uint8,
+                            device=device)
+    args = pack_decode_args(
+        tokens, width, inner, experts, top_k, ROUTING_MODES[mode], int(n_group), int(topk_group), limit is not None,
+        router.dtype == torch.float32, shared_inner, float(routed_scaling), 0.0 if limit is None else float(limit), x.data_ptr(),
+        residual.data_ptr(), router.data_ptr(), 0 if bias is None else bias.data_ptr(), w13.data_ptr(),
+        0 if s13 is None else s13.data_ptr(), w2.data_ptr(), 0 if s2 is None else s2.data_ptr(),
+        0 if shared13 is None else shared13.data_ptr(), 0 if shared2 is None else shared2.data_ptr(), weights.data_ptr(),
         ids.data_ptr(), output.data_ptr(), workspace.data_ptr(), status_block(device).data_ptr())
-    check(lib.b200moe_decode(ctypes.byref(args), _stream()), "moe_decode")
+    check(lib.b200moe_decode(args, _stream()), "moe_decode")
     _count(5 if s13 is None else 6)
     return output, weights, ids
