@@ -279,36 +279,104 @@ __device__ __forceinline__ void load_rows(uint8_t* to, const WeightMaps& maps, u
   for (; row < count; row += 8) load_box(to + row * 128, &maps.flat, full, x, y + row, policy);
 }
 
+// A place in the stream: group of eight columns of an expert, in a block of the down product's columns.
+struct Place {
+  int block, index, group;
+};
+struct Part {  // a CTA's
+  Place from, to;
+};
+
 // Where things are in shared memory behind the stages.
 struct Lists {
+  Part part, down;    // this CTA's of this stream; UP: and of the down product's
+  unsigned long long* totals;  // [warps]
   int* begin;         // [experts with tokens + 1] first row of each
   float* scale;       // [T * K] UP, E4M3: the power of two of each row's token
   uint32_t* mask;     // [E][2] the tokens of each expert
-  int* totals;        // [warps]
   uint16_t* expert;   // [experts with tokens]
   uint16_t* first;    // [E] first row of each
   uint8_t* tokens;    // [T * K]
   __host__ __device__ static int bytes(int T, int E, int K) {
     const int R = T * K, most = E < R ? E : R;
-    return 4 * (most + 1) + 4 * R + 8 * E + 4 * (kStreamThreads / 32) + 2 * (most + E) + R;
+    return 8 * (kStreamThreads / 32) + 4 * (most + 1) + 4 * R + 8 * E + 2 * (most + E) + R;
   }
   __device__ void place(uint8_t* base, int T, int E, int K) {
     const int R = T * K, most = E < R ? E : R;
-    begin = reinterpret_cast<int*>(base);
+    totals = reinterpret_cast<unsigned long long*>(base);
+    begin = reinterpret_cast<int*>(totals + kStreamThreads / 32);
     scale = reinterpret_cast<float*>(begin + most + 1);
     mask = reinterpret_cast<uint32_t*>(scale + R);
-    totals = reinterpret_cast<int*>(mask + 2 * E);
-    expert = reinterpret_cast<uint16_t*>(totals + kStreamThreads / 32);
+    expert = reinterpret_cast<uint16_t*>(mask + 2 * E);
     first = expert + most;
     tokens = reinterpret_cast<uint8_t*>(first + E);
   }
 };
 
-// Rows by expert, in token order inside one; returns the number of experts with tokens.  A token has an expert at most
-// once, so an expert's tokens are a mask of 64 bits and a row's place in them a count of bits: nothing is serial.
-// (One warp that ranked 32 assignments at a time took 5 us longer for 48 tokens of 8.)
-__device__ __forceinline__ int build_lists(const Lists& l, const int* __restrict__ ids, int T, int E, int K,
-                                           int* __restrict__ row_of, const float* __restrict__ token_scale) {
+// What eight columns of an expert with n tokens cost in the stream.  Measured with 16 experts of F = 2048, D = 7168 that all
+// have n tokens, E4M3 (us without the 35 that no column costs): n <= 8 120, 16 180, 24 250, 32 290, 40 410, 64 580.
+// bf16 weights are twice the bytes and as many products.  (64 tokens of E = 256: with columns that all counted alike the
+// CTAs of the up product were ready after 510 to 838 us, those of the experts with most tokens last.)
+__device__ __forceinline__ int weight_of(int n, bool fp8) {
+  const int rest = (n % kPassTokens + 7) / 8;  // groups of eight tokens of the last pass
+  return n / kPassTokens * (fp8 ? 5 : 6) + (rest == 0 ? 0 : fp8 ? 1 + rest : max(2 + rest, 4));
+}
+// ... of the shared expert: bf16, and in the down product with another K.
+template <bool DOWN>
+__device__ __forceinline__ int shared_weight(const DecodeParams& p) {
+  if (p.shared_inner == 0) return 0;
+  const int weight = weight_of(p.T, false);
+  return !DOWN ? weight : min(max((int)(((long long)p.shared_inner * weight + p.F / 2) / p.F), 1), 512);
+}
+
+// The columns are cut between the CTAs by weight, in whole groups of eight, what the lowest box of weights holds: a flat
+// position counts such groups times their weight.  The two ends of this CTA's part:
+template <bool DOWN>
+struct Cut {
+  int routed, shared;  // weights
+  int block[2], flat[2], groups[2];
+  __device__ __forceinline__ Cut(const DecodeParams& p, int all_routed) : routed(all_routed), shared(shared_weight<DOWN>(p)) {
+    const long long total = DOWN ? (long long)(routed + shared) * (p.D / 8)
+                                 : (long long)routed * (p.F / 8) + (long long)shared * (p.shared_inner / 8);
+    const int size = kBlockColumns / 8 * (routed + shared);  // of a whole block
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      flat[i] = (int)(total * (blockIdx.x + i) / gridDim.x);
+      block[i] = DOWN ? flat[i] / size : 0;
+      flat[i] -= block[i] * size;
+      groups[i] = (DOWN ? min(kBlockColumns, p.D - block[i] * kBlockColumns) : p.F) / 8;
+    }
+  }
+  // an end in the shared expert, or behind the last of all
+  __device__ __forceinline__ void last(Part& part, int active) const {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int in = flat[i] - routed * groups[i];
+      if (in >= 0)
+        (i == 0 ? part.from : part.to) = shared ? Place{block[i], active, (in + shared - 1) / shared}
+                                                : Place{block[i], active - 1, groups[i]};
+    }
+  }
+  // an end in the expert in place `index`
+  __device__ __forceinline__ void within(Part& part, int index, int before, int weight) const {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int in = flat[i] - before * groups[i];
+      if (in >= 0 && in < weight * groups[i])
+        (i == 0 ? part.from : part.to) = Place{block[i], index, (in + weight - 1) / weight};
+    }
+  }
+};
+
+// Rows by expert, in token order inside one, and this CTA's part of the stream; returns the number of experts with tokens.
+// A token has an expert at most once, so an expert's tokens are a mask of 64 bits and a row's place in them a count of
+// bits: nothing is serial.  (One warp that ranked 32 assignments at a time took 5 us longer for 48 tokens of 8.)
+// Nothing is divided while the stream is walked either: its ends are found here.
+template <bool DOWN>
+__device__ __forceinline__ int build_lists(Lists& l, const DecodeParams& p, int* __restrict__ row_of,
+                                           const float* __restrict__ token_scale) {
+  const int* __restrict__ ids = p.ids;
+  const int T = p.T, E = p.E, K = p.K;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, R = T * K;
   for (int e = tid; e < 2 * E; e += kStreamThreads) l.mask[e] = 0;
   __syncthreads();
@@ -317,37 +385,47 @@ __device__ __forceinline__ int build_lists(const Lists& l, const int* __restrict
     atomicOr(l.mask + 2 * ids[i] + (token >> 5), 1u << (token & 31));
   }
   __syncthreads();
-  // exclusive sums over the experts of (rows, experts with rows), packed in one word
+  // exclusive sums over the experts of (weight, experts with rows, rows), packed in one word
   const int per = (E + kStreamThreads - 1) / kStreamThreads;
   const auto rows = [&](int e) { return e < E ? __popc(l.mask[2 * e]) + __popc(l.mask[2 * e + 1]) : 0; };
-  int mine = 0;
-  for (int j = 0; j < per; ++j) {
-    const int n = rows(tid * per + j);
-    mine += n ? n | (1 << 16) : 0;
-  }
-  int incl = mine;
+  const auto packed = [&](int n) {
+    return n ? (unsigned long long)weight_of(n, p.fp8) << 32 | 1ull << 16 | (unsigned long long)n : 0ull;
+  };
+  unsigned long long mine = 0;
+  for (int j = 0; j < per; ++j) mine += packed(rows(tid * per + j));
+  unsigned long long incl = mine;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
-    const int v = __shfl_up_sync(0xffffffffu, incl, o);
+    const unsigned long long v = __shfl_up_sync(0xffffffffu, incl, o);
     if (lane >= o) incl += v;
   }
   if (lane == 31) l.totals[warp] = incl;
   __syncthreads();
-  int at = incl - mine, active = 0;
+  unsigned long long at = incl - mine, all = 0;
 #pragma unroll
   for (int w = 0; w < kStreamThreads / 32; ++w) {
-    const int n = l.totals[w];
+    const unsigned long long n = l.totals[w];
     if (w < warp) at += n;
-    active += n;
+    all += n;
   }
-  active >>= 16;
+  const int active = (int)(all >> 16) & 0xffff;
+  const int routed = (int)(all >> 32);
+  const Cut<DOWN> cut(p, routed);
+  const Cut<true> down(p, routed);
+  if (tid == 0) {
+    cut.last(l.part, active);
+    if (!DOWN) down.last(l.down, active);
+  }
   for (int j = 0; j < per; ++j) {
     const int e = tid * per + j, n = rows(e);
     if (n) {
+      const int place = (int)(at >> 16) & 0xffff, before = (int)(at >> 32), weight = weight_of(n, p.fp8);
       l.first[e] = (uint16_t)at;
-      l.expert[at >> 16] = (uint16_t)e;
-      l.begin[at >> 16] = at & 0xffff;
-      at += n | (1 << 16);
+      l.expert[place] = (uint16_t)e;
+      l.begin[place] = (int)at & 0xffff;
+      at += packed(n);
+      cut.within(l.part, place, before, weight);
+      if (!DOWN) down.within(l.down, place, before, weight);
     }
   }
   if (tid == 0) l.begin[active] = R;
@@ -382,27 +460,15 @@ struct Stream {
   const DecodeParams& p;
   const Lists& l;
   const int active;
-  int at, end;             // flat output columns
-  int block, block_end;    // the current block and where it ends
+  const int last;          // experts of a block
+  Place at;
+  const Place& to;
   int waiting;             // tokens of the current expert that need another pass over the same weights
   Piece piece;
 
-  // The columns are cut between the CTAs in whole groups of eight, what a flat box of weights holds.
-  __device__ Stream(const DecodeParams& params, const Lists& lists, int n_active)
-      : p(params), l(lists), active(n_active), waiting(0) {
-    const long long b = blockIdx.x, grid = gridDim.x;
-    const long long total = DOWN ? (long long)p.D * (active + shared_cost())
-                                 : (long long)active * p.F + (long long)shared_cost() * p.shared_inner;
-    at = (int)(total / 8 * b / grid) * 8;
-    end = (int)(total / 8 * (b + 1) / grid) * 8;
-  }
-  // what a column of the shared expert (bf16) costs in columns of the others
-  __device__ int shared_cost() const {
-    if (p.shared_inner == 0) return 0;
-    const int bytes = (p.fp8 ? 2 : 1) * ((p.T + kPassTokens - 1) / kPassTokens);
-    return !DOWN ? bytes : min(max((p.shared_inner * bytes + p.F / 2) / p.F, 1), 64);
-  }
-  __device__ int block_width() const { return DOWN ? min(kBlockColumns, p.D - block * kBlockColumns) : p.F; }
+  __device__ Stream(const DecodeParams& params, const Lists& lists, const Part& part, int n_active)
+      : p(params), l(lists), active(n_active), last(n_active + (params.shared_inner > 0)), at(part.from), to(part.to),
+        waiting(0) {}
   __device__ bool next() {
     if (waiting > 0) {
       piece.begin += piece.n;
@@ -420,37 +486,23 @@ struct Stream {
   // more than a quarter of the stages empty.
   __device__ static int fill(int left, int most) { return left > most / 2 && left < most * 3 / 4 ? most / 2 : min(left, most); }
   __device__ bool next_columns() {
-    const int most = DOWN ? 256 : 128, cost = shared_cost();
-    for (;;) {
-      if (at >= end) return false;
-      const int size = kBlockColumns * (active + cost);  // of a whole block
-      block = DOWN ? at / size : 0;
-      const int width = block_width(), shared_width = DOWN ? width : p.shared_inner;
-      const int base = block * size, routed = base + active * width;
-      block_end = routed + cost * shared_width;
-      if (at < routed) {
-        piece.index = (at - base) / width;
-        const int column = at - base - piece.index * width;
-        piece.first = block * kBlockColumns + column;
-        piece.count = fill(min(width - column, end - at), most);
-        at += piece.count;
-        piece.fp8 = p.fp8;
-        piece.begin = l.begin[piece.index];
-        waiting = l.begin[piece.index + 1] - piece.begin;
-      } else {
-        const int group = cost * 8, stop = min(end, block_end);
-        const int column = (at - routed + group - 1) / group * 8, last = (stop - routed + group - 1) / group * 8;
-        piece.index = active;
-        piece.first = block * kBlockColumns + column;
-        piece.count = fill(last - column, most);
-        at = column + piece.count < last ? routed + cost * (column + piece.count) : stop;
-        if (piece.count <= 0) continue;
-        piece.fp8 = false;
-        piece.begin = 0;
-        waiting = p.T;
-      }
-      break;
+    int columns;
+    for (;; at.group = 0) {
+      const bool ends = at.block == to.block && at.index == to.index;
+      const int width = DOWN ? min(kBlockColumns, p.D - at.block * kBlockColumns) : at.index == active ? p.shared_inner : p.F;
+      columns = (ends ? to.group * 8 : width) - at.group * 8;
+      if (columns > 0) break;
+      if (ends || at.block * kBlockColumns >= p.D) return false;
+      if (++at.index == last) at.index = 0, ++at.block;
     }
+    const bool shared = at.index == active;
+    piece.index = at.index;
+    piece.first = at.block * kBlockColumns + at.group * 8;
+    piece.count = fill(columns, DOWN ? 256 : 128);
+    piece.fp8 = p.fp8 && !shared;
+    piece.begin = shared ? 0 : l.begin[at.index];
+    waiting = shared ? p.T : l.begin[at.index + 1] - piece.begin;
+    at.group += piece.count / 8;
     const int tiles = DOWN ? (piece.count + 15) / 16 : (piece.count + 7) / 8;
     piece.rt_log = tiles <= 1 ? 0 : 32 - __clz(tiles - 1);
     piece.blocks = (inner() * (piece.fp8 ? 1 : 2) + 127) / 128;
@@ -471,7 +523,7 @@ struct Barriers {
 // product are formed, act is scaled and the next kernel starts.
 constexpr long long kPrefetchBytes = 256 << 10;
 __device__ __forceinline__ void prefetch_down(const DecodeParams& p, const Lists& l, int active) {
-  Stream<true> now(p, l, active);
+  Stream<true> now(p, l, l.down, active);
   const long long pitch = (long long)p.F * (p.fp8 ? 1 : 2);
   for (long long left = kPrefetchBytes; left > 0 && now.next();) {
     const int e = now.piece.index;
@@ -495,7 +547,7 @@ __device__ __forceinline__ void keep_full(const DecodeParams& p, const DecodeMap
                                           uint8_t* stages, uint8_t* token_stages, float* weight_scales,
                                           int count, Barriers& bars) {
   const int lane = threadIdx.x & 31, turn = (threadIdx.x >> 5) - kMultiplyWarps;
-  Stream<DOWN> now(p, l, active);
+  Stream<DOWN> now(p, l, l.part, active);
   const uint64_t policy = read_once();
   int slot = 0, stage = 0;
   uint32_t phase = 0;
@@ -690,15 +742,15 @@ stream_kernel(const DecodeParams p, const __grid_constant__ DecodeMaps maps, int
   // DOWN finds the routing finished and waits for act alone (keep_full)
   if (!DOWN) dependency_wait();
   dependency_release();
-  const int active = build_lists(l, p.ids, p.T, p.E, p.K, !DOWN && blockIdx.x == 0 ? p.row_of : nullptr,
-                                 !DOWN && p.fp8 ? p.x16_scale : nullptr);
+  const int active = build_lists<DOWN>(l, p, !DOWN && blockIdx.x == 0 ? p.row_of : nullptr,
+                                       !DOWN && p.fp8 ? p.x16_scale : nullptr);
   if (warp >= kMultiplyWarps) {
     keep_full<DOWN>(p, maps, l, active, shared_memory, token_stages, weight_scales, stages, bars);
     return;
   }
 
   const auto meet_all = [] { named_sync(1, 32 * kMultiplyWarps); };  // the multiplying warps
-  Stream<DOWN> now(p, l, active);
+  Stream<DOWN> now(p, l, l.part, active);
   int slot = 0;
   uint32_t phase = 0;
   bool dead = false;  // a wait ran out: go on to the end without waiting, the status says so
