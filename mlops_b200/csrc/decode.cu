@@ -336,12 +336,13 @@ struct Cut {
   int routed, shared;  // weights
   int block[2], flat[2], groups[2];
   __device__ __forceinline__ Cut(const DecodeParams& p, int all_routed) : routed(all_routed), shared(shared_weight<DOWN>(p)) {
-    const long long total = DOWN ? (long long)(routed + shared) * (p.D / 8)
-                                 : (long long)routed * (p.F / 8) + (long long)shared * (p.shared_inner / 8);
+    const unsigned total = DOWN ? (routed + shared) * (p.D / 8) : routed * (p.F / 8) + shared * (p.shared_inner / 8);  // < 2^31
+    const unsigned each = total / gridDim.x, rest = total - each * gridDim.x;
     const int size = kBlockColumns / 8 * (routed + shared);  // of a whole block
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      flat[i] = (int)(total * (blockIdx.x + i) / gridDim.x);
+    for (int i = 0; i < 2; ++i) {  // total * (block + i) / blocks, without a division of 64 bits
+      const unsigned b = blockIdx.x + i;
+      flat[i] = (int)(each * b + rest * b / gridDim.x);
       block[i] = DOWN ? flat[i] / size : 0;
       flat[i] -= block[i] * size;
       groups[i] = (DOWN ? min(kBlockColumns, p.D - block[i] * kBlockColumns) : p.F) / 8;
