@@ -50,12 +50,16 @@ route_topk_kernel(const float* __restrict__ logits, long long ld, int T, int E, 
                   float* __restrict__ weights, int* __restrict__ ids) {
   const int lane = threadIdx.x & 31;
   const int t = blockIdx.x * kRouteWarps + (threadIdx.x >> 5);
-  dependency_release();
-  dependency_wait();
-  if (t >= T) return;
   const float NEG_INF = __int_as_float(0xff800000);
 
   float x[EPL], sel[EPL], pay[EPL];
+  if (mode == 2) {  // the bias is the caller's: it was there before the kernel in front of this one started
+#pragma unroll
+    for (int j = 0; j < EPL; ++j) sel[j] = bias != nullptr && j * 32 + lane < E ? bias[j * 32 + lane] : 0.0f;
+  }
+  dependency_release();
+  dependency_wait();
+  if (t >= T) return;
   const float* row = logits + (long long)t * ld;
 #pragma unroll
   for (int j = 0; j < EPL; ++j) {
@@ -67,9 +71,9 @@ route_topk_kernel(const float* __restrict__ logits, long long ld, int T, int E, 
 #pragma unroll
     for (int j = 0; j < EPL; ++j) {
       const int e = j * 32 + lane;
-      const float sc = __fdiv_rn(1.0f, 1.0f + expf(-x[j]));
+      const float sc = __frcp_rn(1.0f + expf(-x[j]));
       pay[j] = sc;
-      sel[j] = e < E ? sc + (bias != nullptr ? bias[e] : 0.0f) : NEG_INF;
+      sel[j] = e < E ? sc + sel[j] : NEG_INF;
     }
     if (topk_group < n_group) {
       const int gs = E / n_group;
@@ -92,7 +96,8 @@ route_topk_kernel(const float* __restrict__ logits, long long ld, int T, int E, 
       };
       uint32_t my_group = 0;  // lane g holds the key of group g's score; 0: no such group, or taken
       // groups of 32 experts are the registers themselves, and their maxima do not wait for one another (64 tokens
-      // of 256 experts in 8 groups: 7.2 us instead of 8.3)
+      // of 256 experts in 8 groups: 7.2 us instead of 8.3; 4.9 with the bias read early, a reciprocal in the place
+      // of the division, which rounds 1 / d to the same bits, and no division by the group's size)
       if (gs == 32) {
 #pragma unroll
         for (int j = 0; j < EPL; ++j) {
@@ -125,7 +130,7 @@ route_topk_kernel(const float* __restrict__ logits, long long ld, int T, int E, 
 #pragma unroll
       for (int j = 0; j < EPL; ++j) {
         const int e = j * 32 + lane;
-        if (e < E && !((group_mask >> (e / gs)) & 1u)) sel[j] = NEG_INF;
+        if (e < E && !((group_mask >> (gs == 32 ? j : e / gs)) & 1u)) sel[j] = NEG_INF;
       }
     }
   } else {
