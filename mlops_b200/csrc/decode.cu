@@ -7,6 +7,11 @@
 //   y[t,k] = act[t,k] . W2[e]^T                                          stream_kernel<DOWN>
 //   out[t] = residual[t] + sum_k w[t,k] y[t,k] (+ the shared expert's)   join_kernel
 //
+// Measured (calls one after the other, the bytes of the experts with tokens at 6.56 TB/s in brackets): one token of 8 of
+// 128 experts, D = 2048, F = 768 36 us (6), 48 tokens 139 (89); one token of 8 of 256, D = 7168, F = 2048 with a shared
+// expert 110 (68), 64 tokens 900 (720); 17 tokens of 2 of 8, D = 4096, F = 14336 279 (215).  The chain of six
+// kernels takes 20 us however small the layer is.
+//
 // Bound: HBM.  The weights of the experts that got a token are read once, 3 D F bytes each in E4M3, for one
 // or a few multiplications a byte; everything else is small.  So each product is one stream of weight rows
 // through shared memory (boxes of 128 bytes of K, several stages of 32 KB in flight per SM), and the rows of all
