@@ -658,9 +658,9 @@ __device__ __forceinline__ uint4 load16(uint32_t shared_address) {
 // `a`: this lane's first 16 bytes of the slab, the other eight rows `high` bytes further; `b` + token[i]: its first 16 bytes
 // of tile i of the tokens.  acc[4 i + h], acc[4 i + 2 + h] are the sums of token 8 i + 2 t + h for the lane's two weight
 // rows.
-template <int MOST>
+template <int GROUPS, int MOST>
 __device__ __forceinline__ void multiply_e4m3(uint32_t a_at, int high, float2 s, uint32_t b_at, const uint32_t (&token)[MOST],
-                                              int n, float (&acc)[MOST * 4]) {
+                                              float (&acc)[MOST * 4]) {
   uint32_t a[8][4];
 #pragma unroll
   for (int segment = 0; segment < 2; ++segment) {
@@ -671,25 +671,37 @@ __device__ __forceinline__ void multiply_e4m3(uint32_t a_at, int high, float2 s,
     widen(lo.z, a[j + 2][0], a[j + 2][2]), widen(hi.z, a[j + 2][1], a[j + 2][3]);
     widen(lo.w, a[j + 3][0], a[j + 3][2]), widen(hi.w, a[j + 3][1], a[j + 3][3]);
   }
+  // two groups of tokens at a time, whose sums do not wait for one another
 #pragma unroll
-  for (int i = 0; i < MOST; ++i) {
-    if (i * 8 < n) {
-      const uint32_t at = b_at + token[i];
-      float c[4];
-      const uint4 v0 = load16(at), v1 = load16(at ^ 16);
-      mma_f16_from_zero(c, a[0], v0.x, v0.y);
-      mma_f16(c, a[1], v0.z, v0.w);
-      mma_f16(c, a[2], v1.x, v1.y);
-      mma_f16(c, a[3], v1.z, v1.w);
-      const uint4 v2 = load16(at + 128), v3 = load16((at ^ 16) + 128);
-      mma_f16(c, a[4], v2.x, v2.y);
-      mma_f16(c, a[5], v2.z, v2.w);
-      mma_f16(c, a[6], v3.x, v3.y);
-      mma_f16(c, a[7], v3.z, v3.w);
-      acc[4 * i] = fmaf(c[0], s.x, acc[4 * i]);
-      acc[4 * i + 1] = fmaf(c[1], s.x, acc[4 * i + 1]);
-      acc[4 * i + 2] = fmaf(c[2], s.y, acc[4 * i + 2]);
-      acc[4 * i + 3] = fmaf(c[3], s.y, acc[4 * i + 3]);
+  for (int i = 0; i < GROUPS; i += 2) {
+    constexpr int kTwo = 2;
+    float c[kTwo][4];
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      uint4 v[kTwo];
+#pragma unroll
+      for (int h = 0; h < kTwo; ++h)
+        if (i + h < GROUPS) v[h] = load16(((b_at + token[i + h]) ^ ((q & 1) << 4)) + (q >> 1) * 128);
+#pragma unroll
+      for (int h = 0; h < kTwo; ++h) {
+        if (i + h >= GROUPS) continue;
+        if (q == 0)
+          mma_f16_from_zero(c[h], a[0], v[h].x, v[h].y);
+        else
+          mma_f16(c[h], a[2 * q], v[h].x, v[h].y);
+      }
+#pragma unroll
+      for (int h = 0; h < kTwo; ++h)
+        if (i + h < GROUPS) mma_f16(c[h], a[2 * q + 1], v[h].z, v[h].w);
+    }
+#pragma unroll
+    for (int h = 0; h < kTwo; ++h) {
+      if (i + h >= GROUPS) continue;
+      float* sum = acc + 4 * (i + h);
+      sum[0] = fmaf(c[h][0], s.x, sum[0]);
+      sum[1] = fmaf(c[h][1], s.x, sum[1]);
+      sum[2] = fmaf(c[h][2], s.y, sum[2]);
+      sum[3] = fmaf(c[h][3], s.y, sum[3]);
     }
   }
 }
@@ -789,10 +801,17 @@ stream_kernel(const DecodeParams p, const __grid_constant__ DecodeMaps maps, int
       if (!dead) dead = !mbar_wait_warp(&bars.full[slot], phase, &bars.abort, p.status, 72);
       if (block < blocks) {
         const uint32_t a = a_first + slot * kStageA, b = b_first + slot * p.b_rows * kTokenBytes;
-        if (fp8)
-          multiply_e4m3<MOST>(a, high, reinterpret_cast<const float2*>(weight_scales + slot * kStageScales)[warp], b, token,
-                              n, acc);
-        else
+        if (fp8) {
+          const float2 scale = reinterpret_cast<const float2*>(weight_scales + slot * kStageScales)[warp];
+          if (MOST == 1 || n <= 8)
+            multiply_e4m3<1>(a, high, scale, b, token, acc);
+          else if (n <= 16)
+            multiply_e4m3<MOST < 2 ? MOST : 2>(a, high, scale, b, token, acc);
+          else if (n <= 24)
+            multiply_e4m3<MOST < 3 ? MOST : 3>(a, high, scale, b, token, acc);
+          else
+            multiply_e4m3<MOST>(a, high, scale, b, token, acc);
+        } else
           multiply_bf16<MOST>(a, high, b, token, n, acc);
       }
       __syncwarp();
