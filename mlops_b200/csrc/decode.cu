@@ -8,8 +8,8 @@
 //   out[t] = residual[t] + sum_k w[t,k] y[t,k] (+ the shared expert's)   join_kernel
 //
 // Measured (calls one after the other, the bytes of the experts with tokens at 6.56 TB/s in brackets): one token of 8 of
-// 128 experts, D = 2048, F = 768 36 us (6), 48 tokens 139 (89); one token of 8 of 256, D = 7168, F = 2048 with a shared
-// expert 110 (68), 64 tokens 900 (720); 17 tokens of 2 of 8, D = 4096, F = 14336 279 (215).  The chain of six
+// 128 experts, D = 2048, F = 768 36 us (6), 48 tokens 136 (89); one token of 8 of 256, D = 7168, F = 2048 with a shared
+// expert 110 (68), 64 tokens 915 (720); 17 tokens of 2 of 8, D = 4096, F = 14336 279 (215).  The chain of six
 // kernels takes 20 us however small the layer is.
 //
 // Bound: HBM.  The weights of the experts that got a token are read once, 3 D F bytes each in E4M3, for one
@@ -272,8 +272,8 @@ __device__ __forceinline__ uint64_t read_once() {
 }
 __device__ __forceinline__ void load_box(void* to, const CUtensorMap* map, uint64_t* full, int x, int y, uint64_t policy) {
   asm volatile(
-      "cp.async.bulk.tensor.2d.shared::cta.global.mbarrier::complete_tx::bytes.L2::cache_hint [%0], [%1, {%3, %4}], [%2], %5;" ::"r"(
-          smem_u32(to)),
+      "cp.async.bulk.tensor.2d.shared::cta.global.mbarrier::complete_tx::bytes.L2::cache_hint"
+      " [%0], [%1, {%3, %4}], [%2], %5;" ::"r"(smem_u32(to)),
       "l"(reinterpret_cast<uint64_t>(map)), "r"(smem_u32(full)), "r"(x), "r"(y), "l"(policy)
       : "memory");
 }
@@ -319,7 +319,7 @@ struct Lists {
 };
 
 // What eight columns of an expert with n tokens cost in the stream.  Measured with 16 experts of F = 2048, D = 7168 that all
-// have n tokens, E4M3 (us without the 35 that no column costs): n <= 8 120, 16 180, 24 250, 32 290, 40 410, 64 580.
+// have n tokens, E4M3 (us without the 35 that no column costs): n <= 8 120, 16 160, 24 220, 32 240, 40 350, 64 470.
 // bf16 weights are twice the bytes and as many products.  (64 tokens of E = 256: with columns that all counted alike the
 // CTAs of the up product were ready after 510 to 838 us, those of the experts with most tokens last.)
 __device__ __forceinline__ int weight_of(int n, bool fp8) {
@@ -340,8 +340,10 @@ template <bool DOWN>
 struct Cut {
   int routed, shared;  // weights
   int block[2], flat[2], groups[2];
-  __device__ __forceinline__ Cut(const DecodeParams& p, int all_routed) : routed(all_routed), shared(shared_weight<DOWN>(p)) {
-    const unsigned total = DOWN ? (routed + shared) * (p.D / 8) : routed * (p.F / 8) + shared * (p.shared_inner / 8);  // < 2^31
+  __device__ __forceinline__ Cut(const DecodeParams& p, int all_routed)
+      : routed(all_routed), shared(shared_weight<DOWN>(p)) {
+    const unsigned total =  // < 2^31: weights add up to less than 2^13, groups are at most 2^16
+        DOWN ? (routed + shared) * (p.D / 8) : routed * (p.F / 8) + shared * (p.shared_inner / 8);
     const unsigned each = total / gridDim.x, rest = total - each * gridDim.x;
     const int size = kBlockColumns / 8 * (routed + shared);  // of a whole block
 #pragma unroll
@@ -449,8 +451,8 @@ __device__ __forceinline__ int build_lists(Lists& l, const DecodeParams& p, int*
 }
 
 // A piece of the stream: consecutive output columns of one expert (UP: of the activation, gate and up rows alike; DOWN:
-// of y), at most 128 or 256, and at most kPassTokens of its tokens.  Its rows are cut into 1 << rt_log tiles of 16; a stage has
-// 1 << ks_log K blocks of them.  Slab (K block << rt_log) + tile belongs to the warp of that number.
+// of y), at most 128 or 256, and at most kPassTokens of its tokens.  Its rows are cut into 1 << rt_log tiles of 16; a
+// stage has 1 << ks_log K blocks of them.  Slab (K block << rt_log) + tile belongs to the warp of that number.
 struct Piece {
   int index;         // expert with tokens, or `active` for the shared expert
   int first, count;  // output columns
@@ -488,14 +490,19 @@ struct Stream {
     piece.steps = (piece.blocks + (1 << piece.ks_log) - 1) >> piece.ks_log;
     return true;
   }
-  // Of `left` columns those of a piece: half of `most`, twice the K blocks to a stage, where all of them would leave
-  // more than a quarter of the stages empty.
-  __device__ static int fill(int left, int most) { return left > most / 2 && left < most * 3 / 4 ? most / 2 : min(left, most); }
+  // Of `left` columns those of a piece: half of `most`, twice the K blocks to a stage, where all of them would leave more
+  // than a quarter of the stages empty.  Not where the tokens of two K blocks are more than a stage has room for.
+  __device__ int fill(int left, int most) const {
+    const bool twice = 2 * min(waiting, kPassTokens) <= p.b_rows;
+    return twice && left > most / 2 && left < most * 3 / 4 ? most / 2 : min(left, most);
+  }
   __device__ bool next_columns() {
     int columns;
     for (;; at.group = 0) {
       const bool ends = at.block == to.block && at.index == to.index;
-      const int width = DOWN ? min(kBlockColumns, p.D - at.block * kBlockColumns) : at.index == active ? p.shared_inner : p.F;
+      const int width = DOWN                 ? min(kBlockColumns, p.D - at.block * kBlockColumns)
+                        : at.index == active ? p.shared_inner
+                                             : p.F;
       columns = (ends ? to.group * 8 : width) - at.group * 8;
       if (columns > 0) break;
       if (ends || at.block * kBlockColumns >= p.D) return false;
@@ -504,10 +511,10 @@ struct Stream {
     const bool shared = at.index == active;
     piece.index = at.index;
     piece.first = at.block * kBlockColumns + at.group * 8;
-    piece.count = fill(columns, DOWN ? 256 : 128);
     piece.fp8 = p.fp8 && !shared;
     piece.begin = shared ? 0 : l.begin[at.index];
     waiting = shared ? p.T : l.begin[at.index + 1] - piece.begin;
+    piece.count = fill(columns, DOWN ? 256 : 128);
     at.group += piece.count / 8;
     const int tiles = DOWN ? (piece.count + 15) / 16 : (piece.count + 7) / 8;
     piece.rt_log = tiles <= 1 ? 0 : 32 - __clz(tiles - 1);
@@ -548,7 +555,7 @@ __device__ __forceinline__ void prefetch_down(const DecodeParams& p, const Lists
 // warp w has stages w, w + 4, ...: its first lane sends for the boxes, all its lanes bring the scales and the tokens'
 // columns.  There are at least as many stages as fill warps: a warp that fills stage s has filled s - 4, so
 // s - 4 - count has been read and a wait for s - count cannot take the phase before that one for it.
-template <bool DOWN>
+template <bool DOWN, int MOST>
 __device__ __forceinline__ void keep_full(const DecodeParams& p, const DecodeMaps& maps, const Lists& l, int active,
                                           uint8_t* stages, uint8_t* token_stages, float* weight_scales,
                                           int count, Barriers& bars) {
@@ -568,6 +575,12 @@ __device__ __forceinline__ void keep_full(const DecodeParams& p, const DecodeMap
     const int y = (shared ? 0 : l.expert[piece.index] * (DOWN ? p.D : 2 * p.F)) + piece.first;
     const int block_bytes = kSlab << piece.rt_log;
     const __nv_bfloat16* tokens = !DOWN ? p.x : (shared ? p.act_shared : p.act) + (long long)piece.begin * inner;
+    // Beside E4M3 weights a lane has 16 bytes of every other row of the tokens, at the same places of every stage.  Where a
+    // call can have many rows they are found once: 16 experts with 16 tokens each 192 us instead of 216, with 8 tokens 154
+    // instead of 164.  For the one to eight tokens of a small call that is more than it saves (36.8 us instead of 36.2).
+    const uint8_t* tokens16 = reinterpret_cast<const uint8_t*>(DOWN ? p.act16 + (long long)piece.begin * inner : p.x16);
+    uint32_t offset[kPassTokens / 2];
+    bool placed = false;
     // a lane has the scale of half `lane & 1` of slab `lane >> 1`
     const float* scale = nullptr;
     const int scale_ks = lane >> (1 + piece.rt_log);
@@ -614,11 +627,29 @@ __device__ __forceinline__ void keep_full(const DecodeParams& p, const DecodeMap
                    k < inner);
           }
         } else {
-          for (int i = lane; i < rows * 16; i += 32) {
-            const int at = i >> 4, ks = here == 1 ? 0 : at / piece.n, row = at - ks * piece.n;
-            const long long from = DOWN ? piece.begin + row : l.tokens[piece.begin + row];
-            copy16(b + at * kTokenBytes + (((i & 15) ^ (row & 1)) << 4),
-                   (DOWN ? p.act16 : p.x16) + from * inner + (block0 + ks) * 128 + (i & 15) * 8, true);
+          const uint8_t* from = tokens16 + (long long)block0 * 256;
+          uint8_t* to = b + (lane >> 4) * kTokenBytes + (((lane & 15) ^ (lane >> 4)) << 4);
+          const auto place = [&](int at) {  // in bytes from `from`
+            const int ks = MOST == 1 && ks_count == 1 ? 0 : min(at / piece.n, ks_count - 1);
+            const int row = min(at - ks * piece.n, piece.n - 1);
+            return 2 * ((DOWN ? row : l.tokens[piece.begin + row]) * inner + ks * 128 + (lane & 15) * 8);
+          };
+          if (MOST == 1) {
+            for (int at = lane >> 4; at < rows; at += 2, to += 2 * kTokenBytes) copy16(to, from + place(at), true);
+          } else {
+            if (!placed) {  // (the first weights are on their way)
+              placed = true;
+#pragma unroll
+              for (int j = 0; j < kPassTokens / 2; ++j) {
+                if (2 * j >= piece.n << piece.ks_log) break;
+                offset[j] = place(2 * j + (lane >> 4));
+              }
+            }
+#pragma unroll
+            for (int j = 0; j < kPassTokens / 2; ++j) {
+              if (2 * j >= rows) break;
+              if (2 * j + (lane >> 4) < rows) copy16(to + j * 2 * kTokenBytes, from + offset[j], true);
+            }
           }
         }
         copies_arrive(full);
@@ -655,12 +686,41 @@ __device__ __forceinline__ uint4 load16(uint32_t shared_address) {
   return v;
 }
 
+// The widened slab by GROUPS tiles of eight tokens.
+template <int GROUPS>
+__device__ __forceinline__ void multiply_groups(const uint32_t (&a)[8][4], float2 s, uint32_t b_at, const uint32_t* token,
+                                                float* acc) {
+  float c[GROUPS][4];
+#pragma unroll
+  for (int q = 0; q < 4; ++q) {
+    uint4 v[GROUPS];
+#pragma unroll
+    for (int h = 0; h < GROUPS; ++h) v[h] = load16(((b_at + token[h]) ^ ((q & 1) << 4)) + (q >> 1) * 128);
+#pragma unroll
+    for (int h = 0; h < GROUPS; ++h) {
+      if (q == 0)
+        mma_f16_from_zero(c[h], a[0], v[h].x, v[h].y);
+      else
+        mma_f16(c[h], a[2 * q], v[h].x, v[h].y);
+    }
+#pragma unroll
+    for (int h = 0; h < GROUPS; ++h) mma_f16(c[h], a[2 * q + 1], v[h].z, v[h].w);
+  }
+#pragma unroll
+  for (int h = 0; h < GROUPS; ++h) {
+    acc[4 * h] = fmaf(c[h][0], s.x, acc[4 * h]);
+    acc[4 * h + 1] = fmaf(c[h][1], s.x, acc[4 * h + 1]);
+    acc[4 * h + 2] = fmaf(c[h][2], s.y, acc[4 * h + 2]);
+    acc[4 * h + 3] = fmaf(c[h][3], s.y, acc[4 * h + 3]);
+  }
+}
+
 // `a`: this lane's first 16 bytes of the slab, the other eight rows `high` bytes further; `b` + token[i]: its first 16 bytes
 // of tile i of the tokens.  acc[4 i + h], acc[4 i + 2 + h] are the sums of token 8 i + 2 t + h for the lane's two weight
 // rows.
-template <int GROUPS, int MOST>
-__device__ __forceinline__ void multiply_e4m3(uint32_t a_at, int high, float2 s, uint32_t b_at, const uint32_t (&token)[MOST],
-                                              float (&acc)[MOST * 4]) {
+template <int MOST>
+__device__ __forceinline__ void multiply_e4m3(uint32_t a_at, int high, float2 s, uint32_t b_at,
+                                              const uint32_t (&token)[MOST], int n, float (&acc)[MOST * 4]) {
   uint32_t a[8][4];
 #pragma unroll
   for (int segment = 0; segment < 2; ++segment) {
@@ -671,38 +731,15 @@ __device__ __forceinline__ void multiply_e4m3(uint32_t a_at, int high, float2 s,
     widen(lo.z, a[j + 2][0], a[j + 2][2]), widen(hi.z, a[j + 2][1], a[j + 2][3]);
     widen(lo.w, a[j + 3][0], a[j + 3][2]), widen(hi.w, a[j + 3][1], a[j + 3][3]);
   }
-  // two groups of tokens at a time, whose sums do not wait for one another
-#pragma unroll
-  for (int i = 0; i < GROUPS; i += 2) {
-    constexpr int kTwo = 2;
-    float c[kTwo][4];
-#pragma unroll
-    for (int q = 0; q < 4; ++q) {
-      uint4 v[kTwo];
-#pragma unroll
-      for (int h = 0; h < kTwo; ++h)
-        if (i + h < GROUPS) v[h] = load16(((b_at + token[i + h]) ^ ((q & 1) << 4)) + (q >> 1) * 128);
-#pragma unroll
-      for (int h = 0; h < kTwo; ++h) {
-        if (i + h >= GROUPS) continue;
-        if (q == 0)
-          mma_f16_from_zero(c[h], a[0], v[h].x, v[h].y);
-        else
-          mma_f16(c[h], a[2 * q], v[h].x, v[h].y);
-      }
-#pragma unroll
-      for (int h = 0; h < kTwo; ++h)
-        if (i + h < GROUPS) mma_f16(c[h], a[2 * q + 1], v[h].z, v[h].w);
-    }
-#pragma unroll
-    for (int h = 0; h < kTwo; ++h) {
-      if (i + h >= GROUPS) continue;
-      float* sum = acc + 4 * (i + h);
-      sum[0] = fmaf(c[h][0], s.x, sum[0]);
-      sum[1] = fmaf(c[h][1], s.x, sum[1]);
-      sum[2] = fmaf(c[h][2], s.y, sum[2]);
-      sum[3] = fmaf(c[h][3], s.y, sum[3]);
-    }
+  // two groups of tokens at a time where there are two: their sums do not wait for one another
+  if (MOST == 1 || n <= 8) {
+    multiply_groups<1>(a, s, b_at, &token[0], &acc[0]);
+  } else {
+    multiply_groups<2>(a, s, b_at, &token[0], &acc[0]);
+    if (n > 24)
+      multiply_groups<2>(a, s, b_at, &token[MOST / 2], &acc[4 * (MOST / 2)]);
+    else if (n > 16)
+      multiply_groups<1>(a, s, b_at, &token[MOST / 2], &acc[4 * (MOST / 2)]);
   }
 }
 
@@ -763,7 +800,7 @@ stream_kernel(const DecodeParams p, const __grid_constant__ DecodeMaps maps, int
   const int active = build_lists<DOWN>(l, p, !DOWN && blockIdx.x == 0 ? p.row_of : nullptr,
                                        !DOWN && p.fp8 ? p.x16_scale : nullptr);
   if (warp >= kMultiplyWarps) {
-    keep_full<DOWN>(p, maps, l, active, shared_memory, token_stages, weight_scales, stages, bars);
+    keep_full<DOWN, MOST>(p, maps, l, active, shared_memory, token_stages, weight_scales, stages, bars);
     return;
   }
 
@@ -789,7 +826,7 @@ stream_kernel(const DecodeParams p, const __grid_constant__ DecodeMaps maps, int
 #pragma unroll
     for (int i = 0; i < MOST; ++i) {
       const int j = min(i * 8 + g, piece.n - 1);
-      token[i] = j * pitch + (piece.fp8 ? ((2 * t) ^ (j & 1)) << 4 : t << 4);
+      token[i] = j * pitch + (piece.fp8 ? ((2 * t) ^ ((ks * piece.n + j) & 1)) << 4 : t << 4);
     }
     float acc[MOST * 4];
 #pragma unroll
@@ -801,17 +838,10 @@ stream_kernel(const DecodeParams p, const __grid_constant__ DecodeMaps maps, int
       if (!dead) dead = !mbar_wait_warp(&bars.full[slot], phase, &bars.abort, p.status, 72);
       if (block < blocks) {
         const uint32_t a = a_first + slot * kStageA, b = b_first + slot * p.b_rows * kTokenBytes;
-        if (fp8) {
-          const float2 scale = reinterpret_cast<const float2*>(weight_scales + slot * kStageScales)[warp];
-          if (MOST == 1 || n <= 8)
-            multiply_e4m3<1>(a, high, scale, b, token, acc);
-          else if (n <= 16)
-            multiply_e4m3<MOST < 2 ? MOST : 2>(a, high, scale, b, token, acc);
-          else if (n <= 24)
-            multiply_e4m3<MOST < 3 ? MOST : 3>(a, high, scale, b, token, acc);
-          else
-            multiply_e4m3<MOST>(a, high, scale, b, token, acc);
-        } else
+        if (fp8)
+          multiply_e4m3<MOST>(a, high, reinterpret_cast<const float2*>(weight_scales + slot * kStageScales)[warp], b, token,
+                              n, acc);
+        else
           multiply_bf16<MOST>(a, high, b, token, n, acc);
       }
       __syncwarp();
