@@ -136,6 +136,10 @@ CASES = {
     "bf16, odd tail": dict(T=17, D=72, F=200, E=5, K=5, fp8=False, Fs=24),
     "bf16 router": dict(T=3, D=384, F=128, E=20, K=3, router_dtype=torch.bfloat16),
     "clamped": dict(T=4, D=512, F=256, E=8, K=2, limit=0.5, Fs=128),
+    "24 tokens an expert": dict(T=48, D=1024, F=640, E=8, K=4, Fs=200),
+    "one expert, 64 tokens": dict(T=64, D=1280, F=896, E=1, K=1),
+    "bf16, 48 tokens an expert": dict(T=64, D=520, F=328, E=4, K=3, fp8=False),
+    "256 experts in 8 groups": dict(T=6, D=256, F=128, E=256, K=8, mode="sigmoid_noaux_tc", groups=8, kept=4, scaling=2.5),
     "1000 experts": dict(T=2, D=128, F=128, E=1000, K=32, seed=3),
 }
 
