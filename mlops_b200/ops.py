@@ -1236,8 +1236,8 @@ def moe_decode(x, residual, router, w13, w2, *, top_k, mode, bias=None, n_group=
                             device=device)
     args = pack_decode_args(
         tokens, width, inner, experts, top_k, ROUTING_MODES[mode], int(n_group), int(topk_group), limit is not None,
-        router.dtype == torch.float32, shared_inner, float(routed_scaling), 0.0 if limit is None else float(limit), x.data_ptr(),
-        residual.data_ptr(), router.data_ptr(), 0 if bias is None else bias.data_ptr(), w13.data_ptr(),
+        router.dtype == torch.float32, shared_inner, float(routed_scaling), 0.0 if limit is None else float(limit),
+        x.data_ptr(), residual.data_ptr(), router.data_ptr(), 0 if bias is None else bias.data_ptr(), w13.data_ptr(),
         0 if s13 is None else s13.data_ptr(), w2.data_ptr(), 0 if s2 is None else s2.data_ptr(),
         0 if shared13 is None else shared13.data_ptr(), 0 if shared2 is None else shared2.data_ptr(), weights.data_ptr(),
         ids.data_ptr(), output.data_ptr(), workspace.data_ptr(), status_block(device).data_ptr())
