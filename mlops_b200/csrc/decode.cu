@@ -252,6 +252,9 @@ struct DecodeParams {
   float limit;
   int b_rows;  // capacity of a stage's token part, in rows of one K block
   int* status;
+#ifdef B200_WAIT_TEST
+  int withhold, withheld;  // test builds only: in product 1 (UP) or 2 (DOWN) fill warp `withheld` sends nothing
+#endif
 };
 
 // Weight rows as [experts * rows, K], read in boxes of 128 bytes of K by 8, 32 or all rows of a full piece (UP: 128, DOWN:
@@ -555,6 +558,9 @@ __device__ __forceinline__ void prefetch_down(const DecodeParams& p, const Lists
 // warp w has stages w, w + 4, ...: its first lane sends for the boxes, all its lanes bring the scales and the tokens'
 // columns.  There are at least as many stages as fill warps: a warp that fills stage s has filled s - 4, so
 // s - 4 - count has been read and a wait for s - count cannot take the phase before that one for it.
+// Where a wait runs out: a multiplying warp that has not seen a stage filled no longer says that it has read one, so no
+// slot with copies on their way is filled again (the wait for it ends by the abort flag); and a fill warp leaves, then as
+// always, when its own copies have landed or a bounded wait for them has run out.
 template <bool DOWN, int MOST>
 __device__ __forceinline__ void keep_full(const DecodeParams& p, const DecodeMaps& maps, const Lists& l, int active,
                                           uint8_t* stages, uint8_t* token_stages, float* weight_scales,
@@ -592,7 +598,12 @@ __device__ __forceinline__ void keep_full(const DecodeParams& p, const DecodeMap
               ((long long)l.expert[piece.index] * ((DOWN ? p.D : 2 * p.F) >> 7) + (row >> 7)) * piece.blocks + scale_ks;
     }
     for (int step = 0; step < piece.steps; ++step, ++stage) {
-      if ((stage & (kFillWarps - 1)) == turn) {
+#ifdef B200_WAIT_TEST
+      const bool sends = p.withhold != (DOWN ? 2 : 1) || turn != p.withheld;
+#else
+      constexpr bool sends = true;
+#endif
+      if (sends && (stage & (kFillWarps - 1)) == turn) {
         const int block0 = step << piece.ks_log, here = min(ks_count, piece.blocks - block0);  // K blocks of this stage
         const int rows = here * piece.n;
         if (stage >= count && !mbar_wait_warp(&bars.empty[slot], phase ^ 1, &bars.abort, p.status, 70)) {
@@ -661,15 +672,14 @@ __device__ __forceinline__ void keep_full(const DecodeParams& p, const DecodeMap
     }
   }
   if (!DOWN && turn == 0 && lane == 0) prefetch_down(p, l, active);
-  if (dead) {  // nothing of this warp's may still be on its way when it leaves
-    volatile int go_on = 0;
-    for (int i = 1; i <= min(stage, count); ++i) {
-      slot = slot == 0 ? count - 1 : slot - 1;
-      if (slot == count - 1) phase ^= 1;
-      if (((stage - i) & (kFillWarps - 1)) == turn && lane == 0) mbar_wait(&bars.full[slot], phase, &go_on, p.status, 71);
-    }
-    __syncwarp();
+  // the latest fill of each slot; earlier ones have been read, or the loop has ended in front of them
+  volatile int go_on = 0;
+  for (int i = 1; i <= min(stage, count); ++i) {
+    slot = slot == 0 ? count - 1 : slot - 1;
+    if (slot == count - 1) phase ^= 1;
+    if (((stage - i) & (kFillWarps - 1)) == turn && lane == 0) mbar_wait(&bars.full[slot], phase, &go_on, p.status, 71);
   }
+  __syncwarp();
 }
 
 // One warp's slab of a stage: 16 weight rows x 128 bytes of K by up to 8 * MOST tokens.  Lane (g, t) reads the same
@@ -808,7 +818,7 @@ stream_kernel(const DecodeParams p, const __grid_constant__ DecodeMaps maps, int
   Stream<DOWN> now(p, l, l.part, active);
   int slot = 0;
   uint32_t phase = 0;
-  bool dead = false;  // a wait ran out: go on to the end without waiting, the status says so
+  bool dead = false;  // a wait ran out: go on to the end without waiting or releasing a stage, the status says so
   while (now.next()) {
     const Piece& piece = now.piece;
     const bool is_shared = piece.index == active;
@@ -834,6 +844,8 @@ stream_kernel(const DecodeParams p, const __grid_constant__ DecodeMaps maps, int
     const int n = piece.n, blocks = mine ? piece.blocks : 0;
     const bool fp8 = piece.fp8;
     int block = ks;
+    // No stage is full before act is there; how long that takes is not for the waits below to bound.
+    if (DOWN) dependency_wait();
     for (int step = piece.steps; step > 0; --step, block += ks_count) {
       if (!dead) dead = !mbar_wait_warp(&bars.full[slot], phase, &bars.abort, p.status, 72);
       if (block < blocks) {
@@ -845,7 +857,7 @@ stream_kernel(const DecodeParams p, const __grid_constant__ DecodeMaps maps, int
           multiply_bf16<MOST>(a, high, b, token, n, acc);
       }
       __syncwarp();
-      if (lane == 0) mbar_arrive(&bars.empty[slot]);
+      if (lane == 0 && !dead) mbar_arrive(&bars.empty[slot]);
       if (++slot == stages) {
         slot = 0;
         phase ^= 1;
@@ -1042,6 +1054,16 @@ static int launch_streams(const DecodeParams& p, const DecodeMaps& up, const Dec
 
 using namespace b200;
 
+#ifdef B200_WAIT_TEST
+// Test builds only: which product of the next calls (0: none) lacks the stages of which fill warp; the waits for them run out.
+static int g_withhold_decode[2] = {0, 0};
+extern "C" int b200moe_debug_withhold_decode(int product, int warp) {
+  g_withhold_decode[0] = product;
+  g_withhold_decode[1] = warp;
+  return B200MOE_OK;
+}
+#endif
+
 extern "C" long long b200moe_decode_workspace_bytes(long long tokens, int width, int inner, int experts, int top_k,
                                                     int shared_inner) {
   if (decode_sizes(tokens, width, inner, experts, top_k, shared_inner) != B200MOE_OK) return -1;
@@ -1121,5 +1143,8 @@ extern "C" int b200moe_decode(const b200moe_decode_args* a, void* stream) {
   p.fp8 = fp8, p.limited = a->limited, p.limit = a->limit;
   p.b_rows = p.T <= 2 ? 16 * p.T : kPassTokens;
   p.status = a->status;
+#ifdef B200_WAIT_TEST
+  p.withhold = g_withhold_decode[0], p.withheld = g_withhold_decode[1];
+#endif
   return p.T <= 8 ? launch_streams<1>(p, up, down, s) : launch_streams<kPassTokens / 8>(p, up, down, s);
 }
