@@ -187,7 +187,10 @@ int b200moe_dswiglu_routed(const void* h13, long long ldh, const void* r, long l
  * save8: b200moe_swiglu_quantize (same results, both of which may be NULL) that also writes codes and
  * scales of h13 as it is, before any clamp.
  * restore8: the bf16 values the codes stand for, [rows, 2*width].
- * dswiglu_saved8: b200moe_dswiglu_routed on the values the codes stand for.
+ * dswiglu_saved8: b200moe_dswiglu_routed on the values the codes stand for.  What a block with a NaN scale reaches is
+ * NaN, with a limit too: the activation, the gradients of both halves in its columns, the row's dscore.  (What does
+ * not depend on it stays: without a limit the up half's gradient beside a NaN up block, with one the 0 of a value
+ * of the other half that the limit cuts.)
  */
 int b200moe_swiglu_save8(const void* h13, long long ldh, long long rows, int width, void* act_q, long long ldq,
                          float* scales, long long scale_row_stride, long long scale_block_stride, void* act_bf16,

@@ -415,6 +415,18 @@ __host__ __device__ constexpr uint32_t make_idesc(uint32_t a_fmt, uint32_t b_fmt
 // ----------------------------------------------------------------------------
 // Small numeric helpers
 // ----------------------------------------------------------------------------
+// The smaller and the larger of two, NaN where one is (fminf and fmaxf return the other): a clamp keeps a NaN.
+__device__ __forceinline__ float min_or_nan(float a, float b) {
+  float v;
+  asm("min.NaN.f32 %0, %1, %2;" : "=f"(v) : "f"(a), "f"(b));
+  return v;
+}
+__device__ __forceinline__ float max_or_nan(float a, float b) {
+  float v;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(v) : "f"(a), "f"(b));
+  return v;
+}
+
 __device__ __forceinline__ float warp_max(float v) {
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));

@@ -396,8 +396,13 @@ dswiglu_routed_kernel(const __nv_bfloat16* h13, long long ldh,  // may be the sa
       for (int i = 0; i < 8; ++i) {
         if (!(g[i] <= limit)) keep_g &= ~(1u << i);
         if (!(u[i] >= -limit && u[i] <= limit)) keep_u &= ~(1u << i);
-        g[i] = fminf(g[i], limit);
-        u[i] = fminf(fmaxf(u[i], -limit), limit);
+        if constexpr (SAVED) {
+          g[i] = min_or_nan(g[i], limit);
+          u[i] = min_or_nan(max_or_nan(u[i], -limit), limit);
+        } else {
+          g[i] = fminf(g[i], limit);
+          u[i] = fminf(fmaxf(u[i], -limit), limit);
+        }
       }
     }
     sigmoid8(g, sig);
@@ -419,8 +424,9 @@ dswiglu_routed_kernel(const __nv_bfloat16* h13, long long ldh,  // may be the sa
       if constexpr (LIMITED) {
 #pragma unroll
         for (int h = i; h < i + 2; ++h) {
-          if (!((keep_g >> h) & 1)) dg[h] = 0.f;
-          if (!((keep_u >> h) & 1)) du[h] = 0.f;
+          // a kept value that is NaN stands for one that is not known, nor whether the clamp would have cut it
+          if (!((keep_g >> h) & 1)) dg[h] = SAVED ? 0.f * fabsf(g[h]) : 0.f;
+          if (!((keep_u >> h) & 1)) du[h] = SAVED ? 0.f * fabsf(u[h]) : 0.f;
         }
       }
       amax_g = fmaxf(amax_g, fmaxf(fabsf(dg[i]), fabsf(dg[i + 1])));

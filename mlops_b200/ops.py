@@ -495,7 +495,8 @@ def dswiglu_saved8(saved, r, route_weights, order, *, limit=None, quantized=True
                    scaled_activation=False):
     """`dswiglu_routed` on the pre-activation `swiglu_save8` kept, read in its 8 bits: `(dscore [rows] fp32,
     grad_h13_q, grad_h13_scales, grad_h13_bf16, act_scaled)`. The gradient is that of SwiGLU at the kept
-    values; with a limit, what is clamped goes by them too."""
+    values; with a limit, what is clamped goes by them too. Where a block came back as NaN so does what it reaches,
+    with a limit too: its activation, both halves' gradients in its columns, the row's dscore."""
     return _dswiglu_saved8(*saved, r, route_weights, order, limit, quantized, rounded, scaled_activation)
 
 

@@ -1,0 +1,67 @@
+"""Values that are none beside a clamp: what comes out of a NaN, or of a kept block that a NaN or an infinity made
+unreadable, is a NaN, and never the clamp's border. Comparisons are exact: everything else keeps its bits."""
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda:0"
+
+
+def _ops():
+    from mlops_b200 import ops
+
+    return ops
+
+
+def _bits(t):
+    return t.view(torch.uint8) if t.dtype == torch.float8_e4m3fn else t
+
+
+def _same(a, b):
+    return torch.equal(_bits(a), _bits(b))
+
+
+@pytest.mark.parametrize("limit", [2.0, 1e30])
+@pytest.mark.parametrize("half", [0, 1])
+@pytest.mark.parametrize("bad", [float("nan"), float("inf"), -float("inf")])
+@pytest.mark.parametrize("width,quantized", [(264, False), (384, True)])
+def test_the_clamped_backward_of_an_unreadable_block_is_nan(width, quantized, bad, half, limit):
+    """One value of the middle block of a half is none: its 128 columns are not known any more, nor which of them the
+    clamp would have cut. Their activation, both halves' gradients and the row's dscore are NaN; where the other half's
+    own value, which is known, is cut, its gradient is the 0 it always is."""
+    ops = _ops()
+    g = torch.Generator().manual_seed(width)
+    h = (torch.randn(3, 2 * width, generator=g) * 1.5).bfloat16().to(DEV)
+    r = (torch.randn(3, width, generator=g) * 0.5).bfloat16().to(DEV)
+    weights, order = torch.rand(3, generator=g).to(DEV), torch.tensor([2, 0, 1], dtype=torch.int32, device=DEV)
+    h[1, half * width + 130] = 0
+
+    def backward():
+        saved = ops.swiglu_save8(h, limit=limit, quantized=False)[3]
+        results = ops.dswiglu_saved8(saved, r, weights, order, limit=limit, quantized=quantized, rounded=True,
+                                     scaled_activation=True)
+        return saved, results
+
+    clean_saved, clean = backward()
+    h[1, half * width + 130] = bad
+    saved, (dscore, gq, gs, grad, act) = backward()
+    ops.check_status(DEV)
+    lost = torch.zeros(3, 2 * width, dtype=torch.bool, device=DEV)
+    lost[1, half * width + 128:half * width + 256] = True
+    assert torch.equal(ops.restore8(saved).isnan(), lost)
+    columns = lost[:, :width] | lost[:, width:]
+    codes, scales = clean_saved
+    blocks = scales.shape[1] // 2
+    wide = [scales[:, i * blocks:(i + 1) * blocks].repeat_interleave(128, 1)[:, :width] for i in (0, 1)]
+    values = codes.float() * torch.cat(wide, 1)  # as they are kept, in fp32
+    cut = torch.cat([values[:, :width] > limit, values[:, width:].abs() > limit], 1) & ~lost
+    both = torch.cat([columns, columns], 1) & ~cut
+    assert bool(dscore[1].isnan()) and torch.equal(dscore[[0, 2]], clean[0][[0, 2]])
+    assert torch.equal(act.isnan(), columns) and _same(act[~columns], clean[4][~columns])
+    assert torch.equal(grad.isnan(), both), (grad.isnan() != both).nonzero().tolist()
+    assert _same(grad[~both], clean[3][~both])
+    if quantized:
+        assert torch.equal(gq.float().isnan(), both) and _same(gq[~both], clean[1][~both])
+        kept = ~torch.cat([columns, columns], 1)[:, ::128]
+        assert torch.equal(gs[kept], clean[2][kept])
