@@ -773,8 +773,8 @@ __device__ __forceinline__ void multiply_bf16(uint32_t a_at, int high, uint32_t 
 
 __device__ __forceinline__ float gated(float gate, float up, int limited, float limit) {
   if (limited) {
-    gate = fminf(gate, limit);
-    up = fminf(fmaxf(up, -limit), limit);
+    gate = min_or_nan(gate, limit);
+    up = min_or_nan(max_or_nan(up, -limit), limit);
   }
   return gate * __frcp_rn(1.0f + expf(-gate)) * up;
 }

@@ -65,3 +65,37 @@ def test_the_clamped_backward_of_an_unreadable_block_is_nan(width, quantized, ba
         assert torch.equal(gq.float().isnan(), both) and _same(gq[~both], clean[1][~both])
         kept = ~torch.cat([columns, columns], 1)[:, ::128]
         assert torch.equal(gs[kept], clean[2][kept])
+
+
+@pytest.mark.parametrize("where", ["gate", "up", "shared gate", "shared up"])
+@pytest.mark.parametrize("fp8", [True, False])
+def test_a_nan_weight_of_the_up_product_reaches_its_tokens_through_the_clamp(fp8, where):
+    """`layer.forward_decode` with a limit: one NaN in a gate or up row of an expert (of the shared expert) makes one
+    activation NaN, and with it every output of the expert's tokens (of all); the others keep their bits."""
+    from mlops_b200 import layer
+
+    ops = _ops()
+    g = torch.Generator().manual_seed(11)
+    new = lambda *shape, std=1.0: (torch.randn(*shape, generator=g) * std).bfloat16().to(DEV)  # noqa: E731
+    x, residual, router = new(11, 256), new(11, 256), new(8, 256, std=0.1)
+    w13, w2, shared = new(8, 256, 256, std=0.1), new(8, 256, 128, std=0.1), (new(256, 256, std=0.1), new(256, 128, std=0.1))
+    if fp8:
+        w13, w2 = ops.quantize_blocks(w13), ops.quantize_blocks(w2)
+    call = lambda: layer.forward_decode(x, residual, router, w13, w2, top_k=2, routing_mode="softmax_then_topk",  # noqa: E731
+                                        swiglu_limit=0.5, shared=shared)
+    clean, _, ids = call()
+    assert not bool(clean.isnan().any())
+    row = 77 + (128 if "up" in where else 0)
+    if "shared" in where:
+        shared[0][row, 3] = float("nan")
+        hit = torch.ones(11, dtype=torch.bool, device=DEV)
+    else:
+        if fp8:
+            w13[0].view(torch.uint8)[5, row, 3] = 0x7f
+        else:
+            w13[5, row, 3] = float("nan")
+        hit = (ids == 5).any(1)
+        assert 0 < int(hit.sum()) < 11
+    output, _, again = call()
+    assert torch.equal(again, ids) and bool(output[hit].isnan().all()) and torch.equal(output[~hit], clean[~hit])
+    ops.check_status(DEV)
