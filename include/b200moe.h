@@ -153,7 +153,7 @@ int b200moe_quantize_rows_scatter(const void* x, long long ldx, long long tokens
 /*
  * SwiGLU of h13 = [gate | up] (bf16 [rows, 2*width]) computed in fp32 and rounded once
  * to E4M3 with 1x128 scales (act_q, scales) and/or bf16 (act_bf16); either output may be
- * NULL.  `limited` != 0 caps the gate at `limit` and clips up to [-limit, limit].
+ * NULL.  `limited` != 0 caps the gate at `limit` and clips up to [-limit, limit]; a NaN stays one.
  * Reference: src/mlops/kernels/quack_moe/swiglu_rows.py:246-256 (`swiglu_quantize_rows_fp8`),
  * clamp semantics src/mlops/kernels/moe_reference.py:12-17.
  */
@@ -168,6 +168,7 @@ int b200moe_swiglu_quantize(const void* h13, long long ldh, long long rows, int 
  * outside is reported in `status` and entry 0 is used).  Outputs (each may be NULL):
  *   dscore fp32 [rows] = <r, act>; grad_h13 = dSwiGLU(score * r) as E4M3 + 1x128 scales
  *   ([rows, 2*width], needs width % 128 == 0) and/or bf16; act_scaled = score * act (bf16).
+ * With a limit a value outside the clamp's range, a NaN too, has gradient 0 itself.
  * Reference: src/mlops/kernels/quack_moe/swiglu_rows.py:292-316
  * (`routed_swiglu_rows_backward`).
  */

@@ -1060,8 +1060,8 @@ grouped_gemm_fp8_kernel(const __grid_constant__ CUtensorMap tmap_a,
               g8[i] = __bfloat162float(__float2bfloat16_rn(acc[j + i]));
               u8[i] = __bfloat162float(__float2bfloat16_rn(acc[64 + j + i]));
               if (p.limited) {
-                g8[i] = fminf(g8[i], p.limit);
-                u8[i] = fminf(fmaxf(u8[i], -p.limit), p.limit);
+                g8[i] = min_or_nan(g8[i], p.limit);
+                u8[i] = min_or_nan(max_or_nan(u8[i], -p.limit), p.limit);
               }
             }
             sigmoid8(g8, sig);

@@ -285,8 +285,8 @@ swiglu_quant_kernel(const __nv_bfloat16* __restrict__ h13, long long ldh, long l
     if constexpr (LIMITED) {
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        g[i] = fminf(g[i], limit);
-        u[i] = fminf(fmaxf(u[i], -limit), limit);
+        g[i] = min_or_nan(g[i], limit);
+        u[i] = min_or_nan(max_or_nan(u[i], -limit), limit);
       }
     }
     sigmoid8(g, sig);
@@ -396,13 +396,8 @@ dswiglu_routed_kernel(const __nv_bfloat16* h13, long long ldh,  // may be the sa
       for (int i = 0; i < 8; ++i) {
         if (!(g[i] <= limit)) keep_g &= ~(1u << i);
         if (!(u[i] >= -limit && u[i] <= limit)) keep_u &= ~(1u << i);
-        if constexpr (SAVED) {
-          g[i] = min_or_nan(g[i], limit);
-          u[i] = min_or_nan(max_or_nan(u[i], -limit), limit);
-        } else {
-          g[i] = fminf(g[i], limit);
-          u[i] = fminf(fmaxf(u[i], -limit), limit);
-        }
+        g[i] = min_or_nan(g[i], limit);
+        u[i] = min_or_nan(max_or_nan(u[i], -limit), limit);
       }
     }
     sigmoid8(g, sig);

@@ -99,3 +99,68 @@ def test_a_nan_weight_of_the_up_product_reaches_its_tokens_through_the_clamp(fp8
     output, _, again = call()
     assert torch.equal(again, ids) and bool(output[hit].isnan().all()) and torch.equal(output[~hit], clean[~hit])
     ops.check_status(DEV)
+
+
+@pytest.mark.parametrize("half", [0, 1])
+@pytest.mark.parametrize("save8", [False, True])
+def test_the_clamped_activation_of_a_nan_is_nan(save8, half):
+    """`swiglu_quantize` and `swiglu_save8` with a limit, to E4M3 and to bf16: the element alone, as without a limit."""
+    ops = _ops()
+    g = torch.Generator().manual_seed(3)
+    h = (torch.randn(5, 512, generator=g) * 1.5).bfloat16().to(DEV)
+    call = lambda: (ops.swiglu_save8 if save8 else ops.swiglu_quantize)(h, limit=0.75, rounded=True)[:3]  # noqa: E731
+    h[2, half * 256 + 140] = 0
+    clean_q, clean_scales, clean = call()
+    h[2, half * 256 + 140] = float("nan")
+    q, scales, act = call()
+    lost = torch.zeros(5, 256, dtype=torch.bool, device=DEV)
+    lost[2, 140] = True
+    # an activation of 0 (gate or up 0) is never its block's largest: the scales stay
+    assert torch.equal(act.isnan(), lost) and torch.equal(act[~lost], clean[~lost])
+    assert torch.equal(q.float().isnan(), lost) and _same(q[~lost], clean_q[~lost]) and torch.equal(scales, clean_scales)
+
+
+@pytest.mark.parametrize("half", [0, 1])
+def test_the_clamped_backward_of_a_nan_is_nan_but_for_what_is_cut(half):
+    """`dswiglu_routed` with a limit: dscore and the activation are NaN, and so is the gradient of the half that holds a
+    finite value; a NaN lies outside the clamp's range, so its own gradient is 0, as torch's clamp gives it."""
+    ops = _ops()
+    g = torch.Generator().manual_seed(4)
+    h = torch.randn(4, 256, generator=g).clamp(-0.7, 0.7).bfloat16().to(DEV)  # nothing else is cut
+    r, weights = torch.randn(4, 128, generator=g).bfloat16().to(DEV), torch.rand(4, generator=g).to(DEV)
+    order = torch.arange(4, dtype=torch.int32, device=DEV)
+    call = lambda: ops.dswiglu_routed(h, r, weights, order, limit=0.75, rounded=True, scaled_activation=True)  # noqa: E731
+    clean = call()
+    h[1, half * 128 + 9] = float("nan")
+    dscore, _, _, grad, act = call()
+    value = h.float().requires_grad_(True)
+    gate, up = value[:, :128].clamp(max=0.75), value[:, 128:].clamp(-0.75, 0.75)
+    expected = gate * torch.sigmoid(gate) * up
+    slope, = torch.autograd.grad((weights[:, None] * r.float() * expected).sum(), value)
+    other = torch.zeros(4, 256, dtype=torch.bool, device=DEV)
+    other[1, (1 - half) * 128 + 9] = True
+    assert torch.equal(slope.isnan(), other) and torch.equal(grad.isnan(), other) and float(grad[1, half * 128 + 9]) == 0.0
+    changed = other | h.isnan()
+    assert torch.equal(grad[~changed], clean[3][~changed])
+    assert bool(dscore[1].isnan()) and torch.equal(dscore[[0, 2, 3]], clean[0][[0, 2, 3]])
+    assert torch.equal(act.isnan(), h.isnan()[:, :128] | h.isnan()[:, 128:])
+
+
+def test_the_fused_up_projection_clamps_a_nan_like_the_two_calls():
+    ops = _ops()
+    g = torch.Generator().manual_seed(6)
+    x = torch.randn(40, 256, generator=g).bfloat16().to(DEV)
+    w, ws = ops.quantize_blocks((torch.randn(2, 512, 256, generator=g) * 0.1).bfloat16().to(DEV))
+    w.view(torch.uint8)[0, 30, 7] = 0x7f  # a gate row and an up row of the first group
+    w.view(torch.uint8)[0, 256 + 99, 8] = 0x7f
+    xq, xs = ops.quantize_rows(x)
+    offsets = torch.tensor([0, 23, 40], dtype=torch.int32, device=DEV)
+    h13 = ops.grouped_gemm_fp8(xq, xs, w, ws, offsets)
+    q, scales, act = ops.swiglu_quantize(h13, limit=0.5, rounded=True)
+    fused_h13, fused_q, fused_scales = ops.grouped_gemm_fp8_swiglu(xq, xs, w, ws, offsets, limit=0.5)
+    ops.check_status(DEV)
+    lost = torch.zeros(40, 256, dtype=torch.bool, device=DEV)
+    lost[:23, 30] = lost[:23, 99] = True
+    assert torch.equal(act.isnan(), lost) and torch.equal(q.float().isnan(), lost)
+    assert _same(fused_q, q) and torch.equal(fused_scales, scales)
+    assert torch.equal(fused_h13.view(torch.int16)[~h13.isnan()], h13.view(torch.int16)[~h13.isnan()])
