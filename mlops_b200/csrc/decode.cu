@@ -999,10 +999,11 @@ static int launch_router(const b200moe_decode_args* a, float* logits, __half* x1
   config.numAttrs = 1;
   const auto kernel = a->tokens <= 8 ? router_logits_kernel<W, 1> : a->tokens <= 32 ? router_logits_kernel<W, 4>
                                                                                    : router_logits_kernel<W, 8>;
-  return cudaLaunchKernelEx(&config, kernel, (const __nv_bfloat16*)a->x, (const W*)a->router, (int)a->tokens, a->experts,
-                            a->width, logits, x16, x16_scale) == cudaSuccess
-             ? launch_status()
-             : B200MOE_ERR_LAUNCH;
+  if (cudaLaunchKernelEx(&config, kernel, (const __nv_bfloat16*)a->x, (const W*)a->router, (int)a->tokens, a->experts,
+                         a->width, logits, x16, x16_scale) == cudaSuccess)
+    return B200MOE_OK;
+  cudaGetLastError();  // this call's, reported here
+  return B200MOE_ERR_LAUNCH;
 }
 
 // [rows, k] weights in boxes of `height` rows x 128 bytes
