@@ -1088,6 +1088,9 @@ extern "C" int b200moe_decode(const b200moe_decode_args* a, void* stream) {
   if (fp8 && (a->width % 128 || a->inner % 128)) return B200MOE_ERR_ALIGN;
   for (const void* q : {a->x, a->router, a->w13, a->w2, a->shared_w13, a->shared_w2})
     if ((uintptr_t)q & 15) return B200MOE_ERR_ALIGN;
+  for (const void* q : {(const void*)a->w13_scale, (const void*)a->w2_scale, (const void*)a->bias,
+                        (const void*)a->route_weights, (const void*)a->ids, (const void*)a->status})
+    if ((uintptr_t)q & 3) return B200MOE_ERR_ALIGN;
   if (((uintptr_t)a->workspace & 255) || ((uintptr_t)a->output & 1) || ((uintptr_t)a->residual & 1))
     return B200MOE_ERR_ALIGN;
   if (a->tokens == 0) return B200MOE_OK;
