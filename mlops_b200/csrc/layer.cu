@@ -137,7 +137,7 @@ static int forward_fp8(const b200moe_forward_args* a, bool save, void* codes, fl
     return B200MOE_ERR_ARG;
   if (!all_aligned(16, {a->x, a->residual, a->w13, a->w2, a->h13, a->output, a->x_q, a->act_q, a->expert_rows,
                         codes}) ||
-      !all_aligned(256, {a->workspace}))
+      !all_aligned(4, {code_scales}) || !all_aligned(256, {a->workspace}))
     return B200MOE_ERR_ALIGN;
   const int D = a->width, F = a->inner, E = a->experts, K = a->top_k;
   const long long T = a->tokens, R = T * K;
@@ -190,7 +190,7 @@ static int backward_fp8(const b200moe_backward_args* a, bool saved, const void* 
     return B200MOE_ERR_ARG;
   if (!all_aligned(16, {a->grad_output, a->x, a->w13, a->w2, saved ? codes : a->h13, a->grad_x, a->grad_w13, a->grad_w2, a->dy_q,
                         a->rows, a->r, a->gh_q, a->gh}) ||
-      !all_aligned(256, {a->workspace}))
+      !all_aligned(4, {code_scales}) || !all_aligned(256, {a->workspace}))
     return B200MOE_ERR_ALIGN;
   const int D = a->width, F = a->inner, E = a->experts, K = a->top_k;
   const long long T = a->tokens, R = T * K;

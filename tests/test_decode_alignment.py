@@ -17,3 +17,9 @@ def _filled(struct, sizes, **changes):
 def test_words_at_odd_addresses_are_refused(name):
     sizes = dict(tokens=4, width=256, inner=128, experts=8, top_k=2, mode=1, n_group=1, topk_group=1)
     assert lib.b200moe_decode(_filled(DecodeArgs, sizes, **{name: 4096 + 2}), None) == -2
+
+
+def test_the_one_call_layer_refuses_code_scales_at_an_odd_address_before_it_launches():
+    sizes = dict(tokens=4, width=256, inner=128, experts=8, top_k=2, mode=1)
+    assert lib.b200moe_forward_fp8_save8(_filled(ForwardArgs, sizes), 4096, 4096 + 2, None) == -2
+    assert lib.b200moe_backward_fp8_saved8(_filled(BackwardArgs, sizes, h13=None), 4096, 4096 + 2, None) == -2
