@@ -22,11 +22,11 @@
 //
 // The weights are the A operand of mma.sync.m16n8k16 (16 weight rows), the tokens the B operand (8 to a tile).
 // Against bf16 weights the tokens are bf16.  E4M3 weights are widened to f16, one instruction for two values, and a
-// token is f16 with a power of two of its own that puts its largest value in [2^14, 2^15): every bf16 value down to 2^-29
-// of the largest exactly, what is smaller within 2^-40 of it.  The 128 x 128 block scales are applied in fp32 to the
-// sums of one block, the tokens' powers of two to the finished sums.  (Widening to bf16 takes four
-// instructions for two values, 200 of the 356 issue slots an SM has per 2 KB of weights at full HBM rate;
-// m16n8k32 on E4M3 operands widens them inside, again for every tile: 22 cycles against 8 of m16n8k16.)
+// token is f16 with a power of two of its own that puts its largest value in [2^14, 2^15): every bf16 value down to 2^-31
+// of the largest exactly, what is smaller within 2^-39 of it (half of f16's smallest step, 2^-25, over 2^14).  The
+// 128 x 128 block scales are applied in fp32 to the sums of one block, the tokens' powers of two to the finished sums.
+// (Widening to bf16 takes four instructions for two values, 200 of the 356 issue slots an SM has per 2 KB of weights at
+// full HBM rate; m16n8k32 on E4M3 operands widens them inside, again for every tile: 22 cycles against 8 of m16n8k16.)
 //
 // tcgen05 is not used: it has no product of E4M3 by 16-bit values, its tiles start at 64 rows, and at one to eight tokens
 // a weight row the tensor rate is not what bounds this.  Sums are fp32; act is rounded to bf16 once, as the operand of the
@@ -235,9 +235,8 @@ struct DecodeParams {
   const __nv_bfloat16* residual;
   const int* ids;
   const float* route_weights;
-  const uint8_t *w13, *w2;  // E4M3 or bf16
+  const uint8_t* w2;  // E4M3 or bf16; the products read the weights through tensor maps, this is for prefetch_down
   const float *w13_scale, *w2_scale;
-  const uint8_t *shared_w13, *shared_w2;  // bf16, or null
   const __half* x16;                      // x against E4M3 weights: [T, D], and
   const float* x16_scale;                 // its powers of two
   __nv_bfloat16* act;                     // [T * K, F] in expert order
@@ -1127,12 +1126,9 @@ extern "C" int b200moe_decode(const b200moe_decode_args* a, void* stream) {
   p.residual = reinterpret_cast<const __nv_bfloat16*>(a->residual);
   p.ids = a->ids;
   p.route_weights = a->route_weights;
-  p.w13 = reinterpret_cast<const uint8_t*>(a->w13);
   p.w2 = reinterpret_cast<const uint8_t*>(a->w2);
   p.w13_scale = a->w13_scale;
   p.w2_scale = a->w2_scale;
-  p.shared_w13 = reinterpret_cast<const uint8_t*>(a->shared_w13);
-  p.shared_w2 = reinterpret_cast<const uint8_t*>(a->shared_w2);
   p.x16 = x16;
   p.x16_scale = x16_scale;
   p.act = reinterpret_cast<__nv_bfloat16*>(base + w.act);
