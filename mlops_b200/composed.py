@@ -372,7 +372,8 @@ def apply(h2, residual, router_weight, w13_experts, w2_experts, *, top_k, routin
     limit = None if swiglu_limit is None else float(swiglu_limit)
     base = residual
     if shared_w13 is not None:
-        base = residual + provider.shared_expert(h2, shared_w13, shared_w2, shared_gate_weight, shared_mode, limit)
+        base = residual + provider.shared_expert(h2, shared_w13, shared_w2, shared_gate_weight, shared_mode, limit,
+                                                 saved="bf16")  # this form keeps h13 in bf16 throughout
     rows = h2.numel() // h2.shape[-1]
     normalized = [rows] if lengths is None else [int(v) for v in lengths]
     bias = router_bias if router_bias is not None else torch.empty(0, dtype=torch.float32, device=h2.device)

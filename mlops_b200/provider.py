@@ -620,13 +620,18 @@ def supports(h2, residual, router_weight, w13_experts, w2_experts, **kwargs):
     return SupportResult.yes() if reason is None else SupportResult.no(reason)
 
 
-def shared_expert(h2, shared_w13, shared_w2, shared_gate_weight=None, shared_mode="add", swiglu_limit=None):
+def shared_expert(h2, shared_w13, shared_w2, shared_gate_weight=None, shared_mode="add", swiglu_limit=None,
+                  saved=None):
     """The always-on shared expert, `W2s . swiglu(W13s . x)` (optionally sigmoid-gated), as an
     ordinary differentiable graph: bf16 library GEMMs, as the reference computes it
     (`src/mlops/moe.py:12-37`; it never quantises the shared expert), around this library's
-    SwiGLU operator."""
+    SwiGLU operator. `saved` is the form its pre-activation is kept in, `"bf16"` or `"int8"`; None goes by
+    `set_saved_activations`."""
+    if saved is not None and saved not in layer.SAVED_FORMS:
+        raise ValueError("saved is 'bf16' or 'int8'")
     h13 = torch.nn.functional.linear(h2, shared_w13)
-    act = swiglu_save8(h13, swiglu_limit)[0] if _saves_int8() else swiglu(h13, swiglu_limit)
+    save8 = _saves_int8() if saved is None else saved == "int8"
+    act = swiglu_save8(h13, swiglu_limit)[0] if save8 else swiglu(h13, swiglu_limit)
     shared = torch.nn.functional.linear(act, shared_w2)
     if shared_mode == "sigmoid":
         gate = torch.sigmoid(torch.nn.functional.linear(h2, shared_gate_weight).float())
