@@ -47,6 +47,9 @@ extern "C" {
  * weights fp32 [tokens, top_k] and ids int32 [tokens, top_k], picks in descending
  * selection value, ties to the lowest expert id.  `bias` (fp32 [experts], may be NULL),
  * n_group, topk_group and routed_scaling are read in mode SIGMOID_NOAUX_TC only.
+ * Where the kept groups hold fewer than top_k experts (top_k > topk_group * experts / n_group) the
+ * places left go to the experts outside them, lowest id first, each with its own score: what a
+ * stable sort of selection values gives whose excluded entries are -infinity.
  * NaN selection values rank above every number (the order of a stable descending sort), so
  * ids are always K distinct experts in range; the NaN shows in the weights.
  * Limits: experts <= 1024, top_k <= 32, n_group <= 32 when group selection is active.
@@ -572,7 +575,7 @@ int b200moe_backward_fp8_saved8(const b200moe_backward_args* args, const void* c
 
 /*
  * The whole layer for 1 to 64 tokens, as a serving loop calls it, without anything a backward pass would need:
- * logits = x . bf16(router)^T, the routing of b200moe_route_topk, and
+ * logits = x . bf16(router)^T, the routing of b200moe_route_topk (its ties and its fill-up included), and
  *   output[t] = residual[t] + sum_k w[t,k] W2[e] bf16(swiglu(W13[e] x[t]))  (+ the shared expert with weight 1)
  * with fp32 sums, activations in bf16 and one rounding of the output.  Weights: E4M3 with fp32 scales per
  * 128 x 128 block (both scale pointers; width and inner multiples of 128), or bf16 (both NULL; multiples of 8).

@@ -159,7 +159,8 @@ def check_status(device=None) -> None:
 # ----------------------------------------------------------------------------- routing
 @_on_tensor_device
 def route_topk(logits, top_k, mode, *, bias=None, n_group=1, topk_group=1, routed_scaling=1.0):
-    """(weights fp32 [T,K], ids int32 [T,K]) of fp32 logits [T,E]."""
+    """(weights fp32 [T,K], ids int32 [T,K]) of fp32 logits [T,E]. Where the kept groups hold fewer than `top_k`
+    experts, the places left go to the excluded ones, lowest id first, each with its own score."""
     _need_cuda(logits, bias)
     if logits.dtype != torch.float32 or logits.dim() != 2 or logits.stride(1) != 1:
         raise NativeError("logits must be fp32 [tokens, experts] with unit inner stride")
