@@ -264,6 +264,10 @@ def forward_decode(
         residual = residual.reshape(h2.shape)
     if type(router_weight) not in (torch.Tensor, torch.nn.Parameter):
         router_weight = getattr(router_weight, "_data", router_weight)
+    if router_weight.dtype not in (torch.bfloat16, torch.float32):
+        router_weight = router_weight.to(torch.bfloat16)  # what it is multiplied as
+    if not router_weight.is_contiguous() or router_weight.data_ptr() % 16:
+        router_weight = router_weight.clone(memory_format=torch.contiguous_format)  # (as a view of flat parameters can be)
     if router_bias is not None and router_bias.numel() == 0:
         router_bias = None
     output, weights, ids = ops.moe_decode(

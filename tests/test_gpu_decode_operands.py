@@ -1,0 +1,36 @@
+"""Operands of the layer for a few tokens that `forward_routed` and `provider.apply` take and its kernels do not read as they
+are: they are converted, or the call says what it does not take."""
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda:0"
+
+
+def _inputs(T=5, D=256, F=128, E=8):
+    g = torch.Generator().manual_seed(7)
+    new = lambda *shape, std=1.0: (torch.randn(*shape, generator=g) * std).bfloat16().to(DEV)  # noqa: E731
+    return new(T, D), new(T, D), new(E, D, std=0.1), new(E, 2 * F, D, std=0.1), new(E, D, F, std=0.1)
+
+
+def _off(t, elements=1):
+    """The same values in a piece of a larger buffer that starts at an odd address."""
+    flat = torch.empty(t.numel() + elements, dtype=t.dtype, device=t.device)
+    flat[elements:] = t.reshape(-1)
+    return flat[elements:].view(t.shape)
+
+
+@pytest.mark.parametrize("kind", ["float16", "float64", "strided", "transposed", "odd address", "odd address, fp32"])
+def test_routers_of_other_types_strides_and_addresses(kind):
+    from mlops_b200 import layer
+
+    x, residual, router, w13, w2 = _inputs()
+    call = lambda r: layer.forward_decode(x, residual, r, w13, w2, top_k=2, routing_mode="softmax_then_topk")  # noqa: E731
+    router = router.to(torch.float16).to(torch.bfloat16)  # values that every type holds
+    wide = torch.zeros(8, 512, dtype=torch.bfloat16, device=DEV)
+    wide[:, :256] = router
+    other = {"float16": router.half(), "float64": router.double(), "strided": wide[:, :256],
+             "transposed": router.t().contiguous().t(), "odd address": _off(router),
+             "odd address, fp32": _off(router.float())}[kind]
+    assert all(torch.equal(a, b) for a, b in zip(call(other), call(router)))
