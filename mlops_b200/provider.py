@@ -696,9 +696,10 @@ def decode(h2, residual, router_weight, w13_experts, w2_experts, *, top_k, routi
         raise ValueError(reason)
     shared = None
     if shared_w13 is not None:
-        if shared_mode == "add" and shared_w13.is_contiguous() and shared_w2.is_contiguous():
+        if shared_mode == "add" and all(w.is_contiguous() and w.data_ptr() % 16 == 0 for w in (shared_w13, shared_w2)):
             shared = (shared_w13, shared_w2)
-        else:  # gated, or of strides the kernels do not read
+        else:  # gated, or of strides or at addresses the kernels do not read
+            swiglu_limit = None if swiglu_limit is None else float(swiglu_limit)
             residual = residual + shared_expert(h2, shared_w13, shared_w2, shared_gate_weight, shared_mode, swiglu_limit)
     return layer.forward_decode(
         h2, residual, router_weight, _operands(w13_experts), _operands(w2_experts), top_k=int(top_k),

@@ -34,3 +34,17 @@ def test_routers_of_other_types_strides_and_addresses(kind):
              "transposed": router.t().contiguous().t(), "odd address": _off(router),
              "odd address, fp32": _off(router.float())}[kind]
     assert all(torch.equal(a, b) for a, b in zip(call(other), call(router)))
+
+
+def test_shared_weights_at_odd_addresses():
+    """They take the library products of `apply`, as strided ones do."""
+    from mlops_b200 import provider
+
+    x, residual, router, w13, w2 = _inputs()
+    g = torch.Generator().manual_seed(8)
+    shared = [(torch.randn(*shape, generator=g) * 0.1).bfloat16().to(DEV) for shape in ((128, 256), (256, 64))]
+    call = lambda residual, **kw: provider.decode(x, residual, router, w13, w2, top_k=2,  # noqa: E731
+                                                  routing_mode="softmax_then_topk", swiglu_limit=1, **kw)
+    expected = call(residual + provider.shared_expert(x, *shared, swiglu_limit=1.0))
+    for one, other in ((_off(shared[0]), shared[1]), (shared[0], _off(shared[1], 3))):
+        assert torch.equal(call(residual, shared_w13=one, shared_w2=other), expected)
