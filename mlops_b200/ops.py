@@ -1234,8 +1234,10 @@ def moe_decode(x, residual, router, w13, w2, *, top_k, mode, bias=None, n_group=
     ids = torch.empty((tokens, top_k), dtype=torch.int32, device=device)
     if tokens == 0:
         return output, weights, ids
-    workspace = torch.empty(_decode_workspace(tokens, width, inner, experts, top_k, shared_inner), dtype=torch.uint8,
-                            device=device)
+    size = _decode_workspace(tokens, width, inner, experts, top_k, shared_inner)
+    if size < 0:
+        raise NativeError("D, F and Fs are at most 2^19")
+    workspace = torch.empty(size, dtype=torch.uint8, device=device)
     args = pack_decode_args(
         tokens, width, inner, experts, top_k, ROUTING_MODES[mode], int(n_group), int(topk_group), limit is not None,
         router.dtype == torch.float32, shared_inner, float(routed_scaling), 0.0 if limit is None else float(limit),

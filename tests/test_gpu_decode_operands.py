@@ -48,3 +48,14 @@ def test_shared_weights_at_odd_addresses():
     expected = call(residual + provider.shared_expert(x, *shared, swiglu_limit=1.0))
     for one, other in ((_off(shared[0]), shared[1]), (shared[0], _off(shared[1], 3))):
         assert torch.equal(call(residual, shared_w13=one, shared_w2=other), expected)
+
+
+def test_sizes_past_the_limit_are_named():
+    from mlops_b200 import layer, ops
+
+    x = torch.zeros(1, 2 ** 19 + 8, dtype=torch.bfloat16, device=DEV)
+    router = torch.zeros(1, x.shape[1], dtype=torch.bfloat16, device=DEV)
+    w13 = torch.zeros(1, 16, x.shape[1], dtype=torch.bfloat16, device=DEV)
+    w2 = torch.zeros(1, x.shape[1], 8, dtype=torch.bfloat16, device=DEV)
+    with pytest.raises(ops.NativeError, match="at most"):
+        layer.forward_decode(x, x, router, w13, w2, top_k=1, routing_mode="softmax_then_topk")
