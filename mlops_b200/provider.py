@@ -26,6 +26,7 @@ import os
 import sys
 
 import torch
+import torch.autograd.forward_ad as forward_ad
 from torch.utils.flop_counter import register_flop_formula
 
 from . import layer
@@ -152,8 +153,11 @@ def refusal(h2, residual, router_weight, w13_experts, w2_experts, *, surface="se
     return None
 
 
+_PLAIN_TYPES = (torch.Tensor, torch.nn.Parameter, torch._subclasses.FakeTensor)  # no container, no wrapper
+
+
 def _plain_bf16(weight) -> bool:
-    return type(weight) in (torch.Tensor, torch.nn.Parameter) and weight.dtype == torch.bfloat16 and weight.dim() == 3
+    return type(weight) in _PLAIN_TYPES and weight.dtype == torch.bfloat16 and weight.dim() == 3
 
 
 def _operands(weight):
@@ -560,8 +564,50 @@ def _swiglu_saved8_bwd_flops(codes, code_scales, grad_act, limit, *_rest, out_va
     return 10 * (codes.numel() // 2)
 
 
+# --------------------------------------------------------- the layer for a few tokens, as one operator
+@torch.library.custom_op("b200moe::moe_decode", mutates_args=())
+def moe_decode(h2: torch.Tensor, residual: torch.Tensor, router_weight: torch.Tensor, w13_experts: torch.Tensor,
+               w2_experts: torch.Tensor, router_bias: torch.Tensor, top_k: int, routing_mode: str, n_group: int,
+               topk_group: int, routed_scaling: float, swiglu_limit: float | None, shared_mode: str,
+               shared: list[torch.Tensor], weight_components: list[torch.Tensor]) -> torch.Tensor:
+    """What `decode` runs, where it is traced or counted: `shared` is empty or `[w13, w2]`, with the gate's weight behind
+    them where there is one. (Elsewhere `decode` calls the kernels' wrapper itself: a registered operator takes the
+    host 28 us beside the 35 of that call.)"""
+    with torch.cuda.device(h2.device):
+        return _run_decode(h2, residual, router_weight, *_with_scales(w13_experts, w2_experts, weight_components),
+                           router_bias, top_k, routing_mode, n_group, topk_group, routed_scaling, swiglu_limit,
+                           shared_mode, shared)
+
+
+@moe_decode.register_fake
+def _moe_decode_fake(h2, *_rest):
+    return h2.new_empty(h2.shape)
+
+
+@register_flop_formula(torch.ops.b200moe.moe_decode, get_raw=True)
+def _moe_decode_flops(h2, residual, router_weight, w13_experts, w2_experts, router_bias, top_k, routing_mode, n_group,
+                      topk_group, routed_scaling, swiglu_limit, shared_mode, shared, *_rest, out_val=None, **_kwargs):
+    routed = _logical_flops(h2, router_weight, w13_experts, w2_experts, top_k, True)
+    if not shared:
+        return routed
+    width, inner = shared[1].shape
+    return routed + h2.numel() // h2.shape[-1] * (6 * width * inner + 5 * inner)
+
+
+def _run_decode(h2, residual, router_weight, w13, w2, router_bias, top_k, routing_mode, n_group, topk_group,
+                routed_scaling, swiglu_limit, shared_mode, shared):
+    kernels_read = shared_mode == "add" and all(w.is_contiguous() and w.data_ptr() % 16 == 0 for w in shared[:2])
+    if shared and not kernels_read:  # gated, or of strides or at addresses the kernels do not read
+        residual = residual + shared_expert(h2, shared[0], shared[1], shared[2] if len(shared) > 2 else None,
+                                            shared_mode, swiglu_limit, saved="bf16")
+    return layer.forward_decode(
+        h2, residual, router_weight, w13, w2, top_k=top_k, routing_mode=routing_mode, router_bias=router_bias,
+        n_group=n_group, topk_group=topk_group, routed_scaling=routed_scaling, swiglu_limit=swiglu_limit,
+        shared=tuple(shared[:2]) if shared and kernels_read else None)[0]
+
+
 # ------------------------------------------------------------- containers at the boundary
-_CONTAINER_OPERATORS: list = [moe_fwd, moe_bwd, moe_save8_fwd, moe_saved8_bwd]
+_CONTAINER_OPERATORS: list = [moe_fwd, moe_bwd, moe_save8_fwd, moe_saved8_bwd, moe_decode]
 _DISPATCH_REGISTERED: set = set()
 
 
@@ -688,23 +734,31 @@ def decode(h2, residual, router_weight, w13_experts, w2_experts, *, top_k, routi
                      n_group=n_group, topk_group=topk_group, shared_w13=shared_w13, shared_w2=shared_w2)
     if reason is None and h2.numel() > kernels.DECODE_TOKENS * h2.shape[-1]:
         reason = f"decode takes at most {kernels.DECODE_TOKENS} tokens: apply takes more"
-    if reason is None and torch.is_grad_enabled() and any(
-            t is not None and t.requires_grad for t in (h2, residual, router_weight, w13_experts, w2_experts,
-                                                       shared_w13, shared_w2, shared_gate_weight)):
+    if reason is None and _would_be_differentiated(h2, residual, router_weight, w13_experts, w2_experts, shared_w13,
+                                                   shared_w2, shared_gate_weight):
         reason = "decode has no gradient: call it under torch.no_grad(), or use apply"
     if reason is not None:
         raise ValueError(reason)
-    shared = None
-    if shared_w13 is not None:
-        if shared_mode == "add" and all(w.is_contiguous() and w.data_ptr() % 16 == 0 for w in (shared_w13, shared_w2)):
-            shared = (shared_w13, shared_w2)
-        else:  # gated, or of strides or at addresses the kernels do not read
-            swiglu_limit = None if swiglu_limit is None else float(swiglu_limit)
-            residual = residual + shared_expert(h2, shared_w13, shared_w2, shared_gate_weight, shared_mode, swiglu_limit)
-    return layer.forward_decode(
-        h2, residual, router_weight, _operands(w13_experts), _operands(w2_experts), top_k=int(top_k),
-        routing_mode=str(routing_mode), router_bias=router_bias, n_group=int(n_group), topk_group=int(topk_group),
-        routed_scaling=float(routed_scaling), swiglu_limit=swiglu_limit, shared=shared)[0]
+    shared = [] if shared_w13 is None else [shared_w13, shared_w2] if shared_gate_weight is None \
+        else [shared_w13, shared_w2, shared_gate_weight]
+    limit = None if swiglu_limit is None else float(swiglu_limit)
+    if torch.compiler.is_compiling() or torch._C._len_torch_dispatch_stack() > 0:
+        (w13, *s13), (w2, *s2) = ((w,) if isinstance(w, torch.Tensor) else w
+                                  for w in (_operands(w13_experts), _operands(w2_experts)))
+        bias = router_bias if router_bias is not None else torch.empty(0, dtype=torch.float32, device=h2.device)
+        return moe_decode(h2, residual, router_weight, w13, w2, bias, int(top_k), str(routing_mode), int(n_group),
+                          int(topk_group), float(routed_scaling), limit, str(shared_mode), shared, [*s13, *s2])
+    return _run_decode(h2, residual, router_weight, _operands(w13_experts), _operands(w2_experts), router_bias, int(top_k),
+                       str(routing_mode), int(n_group), int(topk_group), float(routed_scaling), limit, shared_mode, shared)
+
+
+def _would_be_differentiated(*tensors):
+    given = [t for t in tensors if t is not None]
+    if torch.is_grad_enabled() and any(t.requires_grad for t in given):
+        return True
+    # forward mode: a level is open and a tensor carries a tangent
+    return not torch.compiler.is_compiling() and forward_ad._current_level >= 0 \
+        and any(forward_ad.unpack_dual(t).tangent is not None for t in given)
 
 
 def forward(h2, residual, router_weight, w13_experts, w2_experts, *, top_k, routing_mode, router_bias=None,
