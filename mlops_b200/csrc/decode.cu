@@ -8,8 +8,8 @@
 //   out[t] = residual[t] + sum_k w[t,k] y[t,k] (+ the shared expert's)   join_kernel
 //
 // Measured (calls one after the other, the bytes of the experts with tokens at 6.56 TB/s in brackets): one token of 8 of
-// 128 experts, D = 2048, F = 768 36 us (6), 48 tokens 136 (89); one token of 8 of 256, D = 7168, F = 2048 with a shared
-// expert 110 (68), 64 tokens 915 (720); 17 tokens of 2 of 8, D = 4096, F = 14336 279 (215).  The chain of six
+// 128 experts, D = 2048, F = 768 36 us (6), 48 tokens 132 (89); one token of 8 of 256, D = 7168, F = 2048 with a shared
+// expert 110 (68), 64 tokens 870 (720); 17 tokens of 2 of 8, D = 4096, F = 14336 267 (215).  The chain of six
 // kernels takes 20 us however small the layer is.
 //
 // Bound: HBM.  The weights of the experts that got a token are read once, 3 D F bytes each in E4M3, for one

@@ -324,8 +324,9 @@ swiglu_quant_kernel(const __nv_bfloat16* __restrict__ h13, long long ldh, long l
 // these are worked on.  32768 rows of F = 14336 with every output: 1.10 ms (6.0 TB/s); 1.36 ms with
 // scalar arithmetic, which kept the kernel issue-bound.  Three blocks to an SM need 80 registers a
 // thread; at the 83 the compiler takes unasked two fit, and the same took 1.20 ms.  (With a limit 80
-// would spill.)  SAVED reads codes and scales instead of h13: 65536 rows of F = 2048 with every output 308 us (5.3 TB/s;
-// from bf16 305), 8198 rows of F = 14336 282 (from bf16 308): 14 % fewer bytes for as many instructions.
+// would spill.)  SAVED reads codes and scales instead of h13: 65536 rows of F = 2048 with every output 309 us (5.3 TB/s;
+// from bf16 307), 8198 rows of F = 14336 291 (from bf16 303 to 323): 14 % fewer bytes for as many instructions.  (With other
+// rows from call to call the first of these takes 328.)
 template <bool LIMITED, bool SAVED>
 __global__ void __launch_bounds__(kRowWarps * 32, LIMITED ? 2 : 3)
 dswiglu_routed_kernel(const __nv_bfloat16* h13, long long ldh,  // may be the same buffer as gh_bf16

@@ -254,8 +254,10 @@ def forward_decode(
 ) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
     """The layer for 1 to 64 tokens of a serving loop: `(output, route_weights, route_ids)`, arguments as
     `forward_routed` takes them. One host call that reads each needed weight once for every 32 of its tokens;
-    nothing is kept for a backward pass and no statistics are formed. Activations stay bf16 on block-FP8 weights too
-    (`forward_routed` quantises them to E4M3), so the output is the nearer of the two to the weights' exact product.
+    nothing is kept for a backward pass (the results are detached, as `forward_routed`'s are) and no statistics are
+    formed. Activations stay bf16 on block-FP8 weights too (`forward_routed` quantises them to E4M3), so the output is
+    the nearer of the two to the weights' exact product. A router that is not dense, not 16-byte aligned or neither fp32 nor
+    bf16 is copied first.
     `shared = (w13 [2Fs, D], w2 [D, Fs])` (bf16) adds the always-on shared expert."""
     shape = h2.shape
     if len(shape) != 2:

@@ -442,8 +442,8 @@ def swiglu_save8(h13, *, limit=None, quantized=True, rounded=False):
     """`swiglu_quantize` that also keeps h13 for the backward pass in 8 bits: `(act_q, scales, act_bf16,
     (codes, code_scales))`, codes int8 `[rows, 2F]` and one fp32 scale per row, half and 128 columns
     (`[rows, 2 ceil(F / 128)]`, gate's first). The kept values, `restore8((codes, code_scales))`, are within
-    1/254 of a block's largest magnitude; a block with a NaN or an infinity comes back as NaN. The activation
-    is that of `swiglu_quantize`, bit for bit."""
+    1/254 of a block's largest magnitude (of 1e-30 where that is larger); a block with a NaN or an infinity comes
+    back as NaN. The activation is that of `swiglu_quantize`, bit for bit."""
     device = _need_cuda(h13)
     if h13.dtype != torch.bfloat16 or h13.dim() != 2 or h13.shape[1] % 16 or h13.shape[1] == 0 \
             or (h13.shape[0] > 0 and h13.stride(1) != 1):
