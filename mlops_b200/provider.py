@@ -756,9 +756,9 @@ def _would_be_differentiated(*tensors):
     given = [t for t in tensors if t is not None]
     if torch.is_grad_enabled() and any(t.requires_grad for t in given):
         return True
-    # forward mode: a level is open and a tensor carries a tangent
+    # forward mode: a level is open and a tensor carries a tangent (a container cannot)
     return not torch.compiler.is_compiling() and forward_ad._current_level >= 0 \
-        and any(forward_ad.unpack_dual(t).tangent is not None for t in given)
+        and any(type(t) in _PLAIN_TYPES and forward_ad.unpack_dual(t).tangent is not None for t in given)
 
 
 def forward(h2, residual, router_weight, w13_experts, w2_experts, *, top_k, routing_mode, router_bias=None,
