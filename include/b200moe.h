@@ -580,9 +580,10 @@ int b200moe_backward_fp8_saved8(const b200moe_backward_args* args, const void* c
  * with fp32 sums, activations in bf16 and one rounding of the output.  Weights: E4M3 with fp32 scales per
  * 128 x 128 block (both scale pointers; width and inner multiples of 128), or bf16 (both NULL; multiples of 8).
  * experts <= 1024, top_k <= min(experts, 32), tokens <= 64, width, inner and shared_inner <= 2^19.  Every matrix is
- * dense; x and the weights are 16-byte aligned, scales, bias and the 32-bit results 4-byte.  Results repeat bit for bit.  Six launches (five on bf16 weights), all but the first as dependents of
- * the one in front; a wait that ran out is reported in the status block.  Calls that may overlap on the GPU (other
- * streams, replays of graphs) need a workspace each.
+ * dense; x and the weights are 16-byte aligned, scales, bias and the 32-bit results 4-byte.  Results repeat bit for
+ * bit.  Six launches (five on bf16 weights), all but the first as dependents of the one in front; a wait that ran out
+ * is reported in the status block.  Calls that may overlap on the GPU (other streams, replays of graphs) need a
+ * workspace each.
  */
 typedef struct b200moe_decode_args {
   long long tokens;

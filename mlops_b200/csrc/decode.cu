@@ -1055,7 +1055,8 @@ static int launch_streams(const DecodeParams& p, const DecodeMaps& up, const Dec
 using namespace b200;
 
 #ifdef B200_WAIT_TEST
-// Test builds only: which product of the next calls (0: none) lacks the stages of which fill warp; the waits for them run out.
+// Test builds only: which product of the next calls (0: none) lacks the stages of which fill warp; the waits for them run
+// out.
 static int g_withhold_decode[2] = {0, 0};
 extern "C" int b200moe_debug_withhold_decode(int product, int warp) {
   g_withhold_decode[0] = product;
